@@ -16,7 +16,7 @@ from pathlib import Path
 CSRC = Path(__file__).resolve().parent / "csrc"
 LIB_PATH = CSRC / "libdst_b200.so"
 SOURCES = ["api.cu", "format_kernels.cu", "layout_kernels.cu", "gemm_generic.cu", "gemm_decode.cu", "gemm_decode_tq1.cu", "gemm_prefill.cu", "ep_kernels.cu",
-           "moe_kernels.cu", "moe_layer.cu"]
+           "moe_kernels.cu", "moe_layer.cu", "route_group.cu", "adapter_plan.cu", "adapter_gemm.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-shared",
               "-Xcompiler", "-fPIC"]
 
@@ -31,6 +31,7 @@ MAX_TERMS = 4
 MAX_PEERS = 16
 LAYOUT_CANONICAL, LAYOUT_TILED = 0, 1
 SCORE_FUNCS = {"softmax": 0, "sigmoid": 1, "sqrtsoftplus": 2}
+GROUP_SCORES = {"max": 0, "top2": 1}
 
 
 def nvcc_path() -> str:
@@ -66,6 +67,20 @@ class ExpertWeightsC(ctypes.Structure):
 
     _fields_ = [(name, ctypes.c_void_p * MAX_TERMS) for name in ("w13", "s13", "w2", "s2", "w13_decode", "w2_decode")] + \
                [(name, ctypes.c_int64) for name in ("experts", "hidden", "inter")] + [("n_terms", ctypes.c_int), ("fmt", ctypes.c_int)]
+
+
+class AdaptersC(ctypes.Structure):
+    """``dst_adapters`` of ``include/dst_b200.h``."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("a", "b", "scale", "ranks")] + \
+               [(name, ctypes.c_int64) for name in ("matrices_per_slot", "K", "K_padded", "N")] + \
+               [(name, ctypes.c_int) for name in ("rank_padded", "parts", "dtype")]
+
+
+class AdapterRowsC(ctypes.Structure):
+    """``dst_adapter_rows`` of ``include/dst_b200.h``."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("rows", "x_rows", "tiles")] + [("max_tiles", ctypes.c_int64), ("tile", ctypes.c_int)]
 
 
 _SIGNATURES = {
@@ -109,6 +124,20 @@ _SIGNATURES = {
                                                  ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "dst_route_topk": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
                                       ctypes.c_float, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "dst_route_group_topk": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                            ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int,
+                                            ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "dst_adapter_tile_capacity": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
+    "dst_adapter_plan_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
+    "dst_adapter_plan": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
+                                        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+                                        ctypes.c_void_p]),
+    "dst_adapter_plan_experts_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
+    "dst_adapter_plan_experts": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+                                                ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                                ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "dst_adapter_apply": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int,
+                                         ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p]),
     "dst_combine_add": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
                                        ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "dst_ep_combine_pull_add": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,

@@ -39,6 +39,7 @@ import torch
 
 from . import _lib
 from .kernels import ternary_b200 as kb
+from .ternary.adapters import AdapterPlan, LowRankAdapters
 
 
 @dataclass
@@ -95,12 +96,20 @@ class B200Ops:
         return kb._require("auto")
 
     def route(self, logits: torch.Tensor, top_k: int, route_scale: float, renorm: bool = True, score_func: str = "softmax",
-              bias: torch.Tensor | None = None, gate_temp: float = 1.0):
+              bias: torch.Tensor | None = None, gate_temp: float = 1.0, n_groups: int | None = None, topk_groups: int | None = None,
+              group_score: str = "top2"):
         """boilerplate/engine/model.py:389-405 from the gate's logits: scores = f(logits / gate_temp), selection on
-        scores + bias, weights from the unbiased scores."""
+        scores + bias, weights from the unbiased scores.
+
+        ``n_groups``: the experts are that many groups of neighbours and only those of the ``topk_groups`` best groups can be
+        picked; a group counts by its largest selection score (``group_score`` "max") or the sum of its two largest ("top2").
+        Equal groups and experts: the lower one. Picks are those of exact arithmetic: scores near a border are compared in 64
+        bits."""
         lib = self._lib()
         if score_func not in _lib.SCORE_FUNCS:
             raise ValueError(f"score_func must be one of {sorted(_lib.SCORE_FUNCS)}, got {score_func!r}")
+        if n_groups is not None:
+            return self._route_groups(lib, logits, top_k, route_scale, renorm, score_func, bias, gate_temp, n_groups, topk_groups, group_score)
         logits = logits.float().contiguous()
         T, E = logits.shape
         if bias is not None:
@@ -113,6 +122,33 @@ class B200Ops:
             _lib.check(lib.dst_route_topk(logits.data_ptr(), bias.data_ptr() if bias is not None else None, T, E, top_k,
                                           _lib.SCORE_FUNCS[score_func], ctypes.c_float(gate_temp), 1 if renorm else 0,
                                           ctypes.c_float(route_scale), w.data_ptr(), ids.data_ptr(), kb._stream(logits)))
+        return w, ids
+
+    @staticmethod
+    def _route_groups(lib, logits, top_k, route_scale, renorm, score_func, bias, gate_temp, n_groups, topk_groups, group_score):
+        if group_score not in _lib.GROUP_SCORES:
+            raise ValueError(f"group_score must be one of {sorted(_lib.GROUP_SCORES)}, got {group_score!r}")
+        if not logits.is_cuda:
+            raise RuntimeError(kb._UNAVAILABLE + ": router logits are not on a CUDA device")
+        if logits.dtype not in kb._OUT:
+            logits = logits.float()
+        if logits.dim() != 2:
+            raise RuntimeError("router logits are [tokens, experts]")
+        T, E = logits.shape
+        if (E != 1 and logits.stride(1) != 1) or (T > 1 and logits.stride(0) < E):
+            logits = logits.contiguous()
+        if bias is not None:
+            bias = bias.to(device=logits.device, dtype=torch.float32).contiguous()
+            if bias.numel() != E:
+                raise ValueError("the gate bias holds one value per expert")
+        w = torch.empty(T, top_k, dtype=torch.float32, device=logits.device)
+        ids = torch.empty(T, top_k, dtype=torch.int32, device=logits.device)
+        with kb._guard(logits.device):
+            _lib.check(lib.dst_route_group_topk(logits.data_ptr(), kb._OUT[logits.dtype], max(logits.stride(0), E),
+                                                bias.data_ptr() if bias is not None else None, T, E, n_groups,
+                                                n_groups if topk_groups is None else topk_groups, _lib.GROUP_SCORES[group_score], top_k,
+                                                _lib.SCORE_FUNCS[score_func], gate_temp, 1 if renorm else 0, route_scale, w.data_ptr(),
+                                                ids.data_ptr(), kb._stream(logits)))
         return w, ids
 
     def sort(self, ids: torch.Tensor, n_experts: int):
@@ -242,6 +278,28 @@ class B200Ops:
         return y
 
 
+class ExpertAdapters:
+    """The low-rank adapters of a MoE layer's routed experts, for requests with adapters of their own: ``gate_up`` beside the
+    stacked w1 / w3 products and ``down`` beside w2 (``ternary.adapters.LowRankAdapters`` over all experts, bf16). ``rank`` is
+    the largest rank, at most 64. ``MoELayer(x, logits, adapters=..., plan=...)`` applies them."""
+
+    def __init__(self, n_adapters: int, n_experts: int, hidden: int, inter: int, rank: int, device="cuda"):
+        self.gate_up = LowRankAdapters(n_adapters, hidden, 2 * inter, rank, experts=n_experts, parts=2, device=device)
+        self.down = LowRankAdapters(n_adapters, inter, hidden, rank, experts=n_experts, device=device)
+
+    def load(self, slot: int, gate, up, down, scale: float = 1.0) -> None:
+        """Put an adapter into ``slot``: ``gate`` and ``up`` are (A [experts, r, hidden], B [experts, inter, r]) of one rank,
+        ``down`` is (A [experts, r, inter], B [experts, hidden, r]); the added product is scale * B A."""
+        if gate[0].shape != up[0].shape or gate[1].shape != up[1].shape:
+            raise RuntimeError("inconsistent adapter shapes")
+        self.gate_up.load(slot, torch.cat([gate[0], up[0]], 1), torch.cat([gate[1], up[1]], 1), scale)
+        self.down.load(slot, *down, scale)
+
+    def clear(self, slot: int) -> None:
+        self.gate_up.clear(slot)
+        self.down.clear(slot)
+
+
 class MoELayer:
     """Single-device routed-expert layer over ``ExpertWeights``.
 
@@ -253,28 +311,45 @@ class MoELayer:
     Router options of the V4 flavour (model.py:389-405): ``score_func`` "softmax" | "sigmoid" | "sqrtsoftplus",
     ``gate_bias`` [E] added for the selection only, ``gate_temp`` dividing the logits, ``norm_topk_prob``,
     ``route_scale``. ``shared``: the shared expert as ``ExpertWeights`` holding one expert (model.py:421), or None.
+    ``n_groups``, ``topk_groups``, ``group_score``: routing in groups (``B200Ops.route``).
+
+    ``adapters`` and ``plan`` of a call: the requests' low-rank adapters of the routed experts (``ExpertAdapters``) and the
+    batch's ``AdapterPlan``; each of the two expert products is rounded to bf16 after the adapter's part was added. The shared
+    expert has none.
     """
 
     def __init__(self, weights: ExpertWeights, top_k: int, route_scale: float = 1.0, swiglu_limit: float = 0.0, ops=None,
                  flavour: str = "v4", norm_topk_prob: bool = True, score_func: str = "softmax", gate_bias=None,
-                 gate_temp: float = 1.0, shared: ExpertWeights | None = None):
+                 gate_temp: float = 1.0, shared: ExpertWeights | None = None, n_groups: int | None = None, topk_groups: int | None = None,
+                 group_score: str = "top2"):
         if flavour not in ("v4", "standard"):
             raise ValueError(f"flavour must be 'v4' or 'standard', got {flavour!r}")
         if score_func not in _lib.SCORE_FUNCS:
             raise ValueError(f"score_func must be one of {sorted(_lib.SCORE_FUNCS)}, got {score_func!r}")
         if flavour == "standard" and (score_func != "softmax" or gate_bias is not None or gate_temp != 1.0 or shared is not None):
             raise ValueError("the standard flavour routes by plain softmax and has no shared expert (engine/standard.py:156-176)")
+        if n_groups is None and topk_groups is not None:
+            raise ValueError("topk_groups goes with n_groups")
+        if n_groups is not None:
+            kept = n_groups if topk_groups is None else topk_groups
+            if flavour == "standard" or group_score not in _lib.GROUP_SCORES or not 1 <= kept <= n_groups <= 32:
+                raise ValueError("routing in groups: the v4 flavour, at most 32 groups, topk_groups of them, "
+                                 f"group_score one of {sorted(_lib.GROUP_SCORES)}")
         if shared is not None and (shared.n_experts != 1 or shared.hidden != weights.hidden):
             raise ValueError("the shared expert is one expert over the same hidden size")
         self.w, self.top_k, self.route_scale, self.swiglu_limit = weights, top_k, route_scale, swiglu_limit
         self.flavour, self.norm_topk_prob = flavour, norm_topk_prob
         self.score_func, self.gate_bias, self.gate_temp, self.shared = score_func, gate_bias, gate_temp, shared
+        self.n_groups, self.topk_groups, self.group_score = n_groups, topk_groups, group_score
         self.ops = ops if ops is not None else B200Ops()
 
     def route(self, logits: torch.Tensor):
         """(weights [T, k] f32, ids [T, k]) from the gate's logits, per this layer's router options."""
         if self.flavour == "standard":
             return self.ops.route(logits, self.top_k, 1.0, renorm=self.norm_topk_prob)
+        if self.n_groups is not None:
+            return self.ops.route(logits, self.top_k, self.route_scale, renorm=self.norm_topk_prob, score_func=self.score_func, bias=self.gate_bias,
+                                  gate_temp=self.gate_temp, n_groups=self.n_groups, topk_groups=self.topk_groups, group_score=self.group_score)
         if self.score_func == "softmax" and self.gate_bias is None and self.gate_temp == 1.0:
             if self.norm_topk_prob:
                 return self.ops.route(logits, self.top_k, self.route_scale)  # the three-argument form every ops object has
@@ -290,6 +365,27 @@ class MoELayer:
         h = self.ops.swiglu_std(gu, w.inter, for_weights=self._for_weights(w.w2_packed, w.w2_scale))
         down = self.ops.gemm(h, offsets, w.w2_packed, w.w2_scale, w.inter, w.group, w.fmt)
         return self.ops.combine_weighted(down, order, ids, weights, T, self.top_k)
+
+    def _forward_adapted(self, x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, adapters: ExpertAdapters,
+                         plan: AdapterPlan) -> torch.Tensor:
+        """The layer with the requests' adapters beside its two expert products. The plan's order of the pairs sorts them by
+        expert too, so the grouped products, the gather and the combine use it as it is."""
+        w, ops, T = self.w, self.ops, x.size(0)
+        pairs = plan.for_experts(ids, w.n_experts)
+        xs = self.gather_for_experts(x, pairs.order, self.top_k)
+        gu = torch.empty(T * self.top_k, 2 * w.inter, dtype=torch.float32, device=x.device)
+        ops.gemm(xs, pairs.offsets, w.w13_packed, w.w13_scale, w.hidden, w.group, w.fmt, out=gu)
+        gu = adapters.gate_up(x, pairs, base=gu, out_dtype=torch.bfloat16)
+        if self.flavour == "standard":
+            h = ops.swiglu_std(gu, w.inter)
+        else:
+            h = ops.swiglu(gu, weights.reshape(-1).float().contiguous(), pairs.order, w.inter, self.swiglu_limit)
+        down = torch.empty(T * self.top_k, w.hidden, dtype=torch.float32, device=x.device)
+        ops.gemm(h, pairs.offsets, w.w2_packed, w.w2_scale, w.inter, w.group, w.fmt, out=down)
+        down = adapters.down(h, pairs, base=down, out_dtype=torch.bfloat16, pair_rows=True)
+        if self.flavour == "standard":
+            return ops.combine_weighted(down, pairs.order, ids, weights, T, self.top_k)
+        return ops.combine(down, pairs.order, ids, T, self.top_k, add=self.shared_forward(x))
 
     def experts_forward(self, xs: torch.Tensor, offsets: torch.Tensor, row_weights, order, out=None, weights=None,
                         n_rows_dev=None, scatter=None) -> torch.Tensor:
@@ -390,12 +486,17 @@ class MoELayer:
                                          pw, ps, y.data_ptr(), ws.data_ptr(), nbytes, kb._stream(x)))
         return y
 
-    def forward_routed(self, x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
+    def forward_routed(self, x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, adapters: ExpertAdapters | None = None,
+                       plan: AdapterPlan | None = None) -> torch.Tensor:
         """x [T, hidden] bf16 with routing weights [T, k] f32 and expert ids [T, k] (int32 or int64) that the caller
         computed (``V4Model.route`` / the top-k of ``StandardDecoder._moe``) -> y [T, hidden] bf16. An id outside
         [0, E) drops that (token, slot)."""
         if tuple(weights.shape) != tuple(ids.shape) or weights.size(0) != x.size(0) or weights.size(-1) != self.top_k:
             raise ValueError("weights and ids are [tokens, top_k]")
+        if (adapters is None) != (plan is None):
+            raise ValueError("adapters and plan go together")
+        if adapters is not None:
+            return self._forward_adapted(x, weights, ids, adapters, plan)
         y = self._layer_call(x, weights, ids)
         if y is not None:
             return y
@@ -409,11 +510,14 @@ class MoELayer:
             return self.ops.combine(down, order, ids, T, self.top_k)
         return self.ops.combine(down, order, ids, T, self.top_k, add=self.shared_forward(x))
 
-    def forward(self, x: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, logits: torch.Tensor, adapters: ExpertAdapters | None = None,
+                plan: AdapterPlan | None = None) -> torch.Tensor:
         """x [T, hidden] bf16, router logits [T, E] f32 (``F.linear(x.float(), gate_w)``, before the temperature)
         -> y [T, hidden] bf16."""
         weights, ids = self.route(logits)
-        return self.forward_routed(x, weights, ids)
+        if adapters is None and plan is None:
+            return self.forward_routed(x, weights, ids)
+        return self.forward_routed(x, weights, ids, adapters, plan)
 
     __call__ = forward
 
@@ -496,7 +600,7 @@ class ExpertParallelMoE:
     def __init__(self, weights: ExpertWeights, n_experts_total: int, top_k: int, group=None, route_scale: float = 1.0,
                  swiglu_limit: float = 0.0, ops=None, transport: str = "auto", norm_topk_prob: bool = True,
                  score_func: str = "softmax", gate_bias=None, gate_temp: float = 1.0, shared: ExpertWeights | None = None,
-                 combine: str = "auto"):
+                 combine: str = "auto", n_groups: int | None = None, topk_groups: int | None = None, group_score: str = "top2"):
         """``transport``: "nccl" = all_to_all_single of rows both ways (any backend, also gloo on CPU);
         "peer" = the rows are written into / read from the owners' buffers by this library's kernels over NVLink
         (CUDA, one node, torch symmetric memory, B200Ops); "auto" = "peer" where it can be set up, else "nccl".
@@ -504,7 +608,7 @@ class ExpertParallelMoE:
         slot of the rank that owns the token, over NVLink, while the tensor pipe works on the next tile, and the
         combine is local; "pull" = the GEMM writes locally and each rank reads its tokens' rows from the owners;
         "auto" = "scatter" (measured per step: 3.22 against 3.37 ms at 2 ranks).
-        Router options and ``shared`` as in ``MoELayer`` (``gate_bias`` over the GLOBAL experts; the shared expert is
+        Router options and ``shared`` as in ``MoELayer`` (``gate_bias`` and the groups over the GLOBAL experts; the shared expert is
         replicated: every rank applies it to its own tokens)."""
         import torch.distributed as dist
 
@@ -517,7 +621,8 @@ class ExpertParallelMoE:
         if weights.n_experts != self.El:
             raise ValueError(f"rank holds {weights.n_experts} experts, expected {self.El}")
         self.local = MoELayer(weights, top_k, route_scale, swiglu_limit, ops, norm_topk_prob=norm_topk_prob, score_func=score_func,
-                              gate_bias=gate_bias, gate_temp=gate_temp, shared=shared)
+                              gate_bias=gate_bias, gate_temp=gate_temp, shared=shared, n_groups=n_groups, topk_groups=topk_groups,
+                              group_score=group_score)
         self.ops = self.local.ops
         self.top_k = top_k
         self.last_dispatch_rows = 0

@@ -152,9 +152,20 @@ class TernaryLinear:
             w = d if w is None else w + d
         return w
 
-    def __call__(self, x: torch.Tensor, out_dtype=torch.bfloat16) -> torch.Tensor:
+    def __call__(self, x: torch.Tensor, out_dtype=torch.bfloat16, adapters=None, plan=None) -> torch.Tensor:
+        """``adapters``, ``plan``: the requests' low-rank adapters of this projection (``ternary.adapters``), added to its
+        float32 rows before the one rounding to ``out_dtype``."""
         if not x.is_cuda:
             raise RuntimeError("B200 ternary kernel unavailable for CPU tensors (this backend has no CPU path)")
+        if (adapters is None) != (plan is None):
+            raise ValueError("adapters and plan go together")
+        if adapters is not None:
+            if (adapters.K, adapters.N) != (self.K, self.out_features):
+                raise RuntimeError("inconsistent adapter shapes")
+            base = self(x, torch.float32)
+            od = out_dtype if out_dtype in kb._OUT else torch.float32
+            y = adapters(x.reshape(-1, self.K).to(adapters.dtype), plan, base=base.view(-1, self.out_features), out_dtype=od)
+            return y.view(base.shape).to(out_dtype)
         shape = x.shape
         x2 = x.reshape(-1, self.K)
         laid = self._layout(x2.device)

@@ -202,6 +202,18 @@ int dst_route_softmax_topk(const float* logits, int64_t T, int64_t E, int top_k,
 enum { DST_SCORE_SOFTMAX = 0, DST_SCORE_SIGMOID = 1, DST_SCORE_SQRTSOFTPLUS = 2 };
 int dst_route_topk(const float* logits, const float* bias, int64_t T, int64_t E, int top_k, int score_func, float gate_temp,
                    int renorm, float route_scale, float* weights, int32_t* ids, dst_stream_t stream);
+/*
+ * Routing in groups: the E experts are n_groups groups of E / n_groups consecutive ids. key = score + bias[e] (bias NULL: the
+ * score); a group's score is its largest key (DST_GROUP_MAX) or the sum of its two largest (DST_GROUP_TOP2); the topk_groups
+ * groups of the largest scores stay (equal: the lower group first), and the top_k largest keys of their experts are picked as
+ * dst_route_topk picks them. Picks and their order are those of exact arithmetic (near a border scores are compared in 64
+ * bits); weights as in dst_route_topk. logits [T, E] of DST_OUT_* type logits_dtype, row_stride elements from row to row.
+ * E <= 1024, n_groups <= 32 dividing E, top_k <= 8 and <= topk_groups * E / n_groups, gate_temp != 0.
+ */
+enum { DST_GROUP_MAX = 0, DST_GROUP_TOP2 = 1 };
+int dst_route_group_topk(const void* logits, int logits_dtype, int64_t row_stride, const float* bias, int64_t T, int64_t E, int n_groups,
+                         int topk_groups, int group_score, int top_k, int score_func, float gate_temp, int renorm, float route_scale,
+                         float* weights, int32_t* ids, dst_stream_t stream);
 /* The same with the renormalisation optional (renorm = 0: the softmax scores of the selected experts as they are):
  * the `norm_topk_prob` switch of boilerplate/engine/standard.py:159-165. */
 int dst_route_softmax_topk_ex(const float* logits, int64_t T, int64_t E, int top_k, int renorm, float route_scale,
@@ -270,6 +282,60 @@ size_t dst_moe_layer_workspace_bytes(int64_t T, int top_k, int standard, const d
 int dst_moe_layer(const void* x_bf16, const float* weights, const int32_t* ids, int64_t T, int top_k, int standard, float limit,
                   const dst_expert_weights* w, const dst_expert_weights* shared, void* y_bf16, void* workspace, size_t workspace_bytes,
                   dst_stream_t stream);
+
+/*
+ * Low-rank adapters of many requests beside a projection. The rows of a batch belong to requests, a request has one of n
+ * adapters or none. A plan sorts the rows by adapter, once per batch; it serves every projection of the step.
+ *
+ * dst_adapter_plan: request i has rows offsets[i] .. offsets[i + 1] (device int32 [requests + 1], nondecreasing; NULL: request i
+ * is row i) and adapter slots[i] (outside [0, n): none). Rows behind the last request have none. Written: order [rows] (row of
+ * each position; adapters 0 .. n-1, then the rows without one, each in row order), bins [rows] (the position's adapter, n:
+ * none), bin_offsets [n + 2] (where each adapter's positions start, then those without one, then rows), tiles
+ * [dst_adapter_tile_capacity(rows, n + 1, tile)], 8-byte aligned: the positions cut into tiles of at most `tile` rows of one
+ * adapter. n <= 4095. Workspace: dst_adapter_plan_workspace_bytes (0 up to 16384 rows and 1023 adapters).
+ *
+ * dst_adapter_plan_experts: the (token, choice) pairs of a MoE layer, ids [T, top_k], sorted by expert and inside an expert by
+ * adapter, from the tokens' plan (order, bins). pair_order [T * top_k] = token * top_k + choice per position (-1 behind the
+ * last pair: ids outside [0, E) are dropped), offsets [E + 1] the experts' first positions: what the grouped GEMM, the gather
+ * and the combine take as order and offsets. x_rows [T * top_k] = the position's token. tiles
+ * [dst_adapter_tile_capacity(T * top_k, (n + 1) * E, tile)]: matrix adapter * E + expert. E <= 4096.
+ */
+int64_t dst_adapter_tile_capacity(int64_t rows, int64_t bins, int tile);
+size_t dst_adapter_plan_workspace_bytes(int64_t rows, int64_t n);
+int dst_adapter_plan(const int32_t* offsets, const int32_t* slots, int64_t requests, int64_t rows, int64_t n, int tile, int32_t* order,
+                     int32_t* bins, int32_t* bin_offsets, int32_t* tiles, void* workspace, size_t workspace_bytes, dst_stream_t stream);
+size_t dst_adapter_plan_experts_workspace_bytes(int64_t pairs, int64_t E);
+int dst_adapter_plan_experts(const int32_t* ids, int64_t T, int top_k, int64_t E, const int32_t* order, const int32_t* bins, int64_t n, int tile,
+                             int64_t* pair_order, int64_t* offsets, int32_t* x_rows, int32_t* tiles, void* workspace, size_t workspace_bytes,
+                             dst_stream_t stream);
+
+/*
+ * out[r, :] = round(base[r, :] + scale[a] * B_m (A_m x[x(r), :])) for the rows of adapter a, round(base[r, :]) for rows without
+ * one; rows that no tile holds are not written. A_m [parts * rank_padded, K_padded] and B_m [N, rank_padded] of matrix m
+ * (dtype DST_ACT_BF16 or DST_ACT_F16, as x), zero behind K, 16-byte aligned; part p of the columns (N / parts each) takes rows
+ * p * rank_padded .. of A. matrices_per_slot: matrices of one adapter (experts; 1 beside a dense projection), adapter
+ * a = m / matrices_per_slot with the rank ranks[a] <= rank_padded; what lies behind it is finite and counts for nothing (rank 0:
+ * the base alone). rank_padded 16, 32, 64 or 128; parts 1 or 2 with parts * rank_padded <= 128; K_padded a multiple of 32.
+ * rows / x_rows: base / out row and x row of a position (NULL: the position). base (DST_OUT_* type) may be NULL (zeros) or the
+ * same rows as out; x may not overlap out. Strides in elements.
+ */
+typedef struct dst_adapters {
+  const void* a;
+  const void* b;
+  const float* scale;
+  const int32_t* ranks;
+  int64_t matrices_per_slot, K, K_padded, N;
+  int rank_padded, parts, dtype;
+} dst_adapters;
+typedef struct dst_adapter_rows {
+  const int32_t* rows;
+  const int32_t* x_rows;
+  const int32_t* tiles;
+  int64_t max_tiles;
+  int tile;
+} dst_adapter_rows;
+int dst_adapter_apply(const dst_adapters* w, const dst_adapter_rows* plan, const void* x, int64_t x_stride, const void* base, int base_dtype,
+                      int64_t base_stride, void* out, int out_dtype, int64_t out_stride, dst_stream_t stream);
 
 /* The same with one more bf16 row per token added in fp32 after the experts' rows and before the cast: the shared
  * expert's output, `y += self.swiglu(L.shared, x)` of boilerplate/engine/model.py:421. add_bf16 [T, hidden] or NULL.

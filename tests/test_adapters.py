@@ -1,0 +1,711 @@
+"""Routing in groups, row plans and low-rank adapters: each against a plain implementation in 64 bits, their refusals, and an
+adapted MoE layer as a whole.
+
+Tolerances. A 16-bit result is off by half a step, eps / 2 of its value. h = A x sums K exact products in float32, at worst one
+instruction of 16 after the other, each within 2^-22 of the sums so far (the adders of the matrix instructions truncate), then
+at most 64 partial sums; the second product adds rank terms alike, and h enters it as pieces that leave 2^-17 of it (16-bit
+results) or 2^-22 (float32 ones, fp16's two pieces). All of that scales with S = |scale| * |B| (|A| |x|), the products' absolute
+values: (K / 16 + 64 + rank) * 2^-22 + pieces. base + product is one float32 rounding more, 2^-23 of the result at most."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from deepseekternarized_b200 import _lib
+from deepseekternarized_b200.kernels import ternary_b200 as kb
+from deepseekternarized_b200.moe import B200Ops, ExpertAdapters, ExpertWeights, MoELayer
+from deepseekternarized_b200.ternary import ops as tops
+from deepseekternarized_b200.ternary.adapters import AdapterPlan, LowRankAdapters
+from deepseekternarized_b200.ternary.pack import pack
+
+gpu = pytest.mark.gpu
+DEV = "cuda"
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+# ------------------------------------------------------------------------------------------------- routing in groups
+def route64(logits, k, scale, renorm, score, bias, temp, groups, kept, group_score):
+    """The definition on the CPU in 64 bits; NaN first, equal keys by the lower index."""
+    v = logits.double().cpu() / float(np.float32(temp))
+    T, E = v.shape
+    s = {"softmax": lambda: torch.softmax(v, -1), "sigmoid": lambda: torch.sigmoid(v),
+         "sqrtsoftplus": lambda: torch.logaddexp(v, torch.zeros_like(v)).sqrt()}[score]()
+    key = s if bias is None else s + bias.double().cpu()
+    w, ids = np.empty((T, k)), np.empty((T, k), np.int64)
+    size = E // groups
+
+    def first(values):  # positions in descending order: NaN, then numbers; stable
+        return sorted(range(len(values)), key=lambda i: (0, 0.0) if np.isnan(values[i]) else (1, -values[i]))
+
+    for t in range(T):
+        row = key[t].numpy()
+        g = []
+        for i in range(groups):
+            part = row[i * size:(i + 1) * size]
+            best = [part[j] for j in first(part)[:2 if group_score == "top2" else 1]]
+            g.append(np.nan if np.isnan(sum(best)) else float(sum(best)))
+        allowed = sorted(first(g)[:kept])
+        cand = [i * size + j for i in allowed for j in range(size)]
+        pick = [cand[j] for j in first(row[cand])[:k]]
+        ids[t] = pick
+        w[t] = s[t].numpy()[pick]
+        if renorm and k > 1:
+            w[t] /= w[t].sum() + 1e-20
+    return w * scale, ids
+
+
+def check_route(logits, k, scale=1.0, renorm=True, score="sigmoid", bias=None, temp=1.0, groups=8, kept=4, group_score="top2"):
+    w, ids = B200Ops().route(logits, k, scale, renorm=renorm, score_func=score, bias=bias, gate_temp=temp, n_groups=groups,
+                             topk_groups=kept, group_score=group_score)
+    want, want_ids = route64(logits, k, scale, renorm, score, bias, temp, groups, kept, group_score)
+    assert np.array_equal(ids.cpu().numpy(), want_ids)
+    # an exponent's argument may be rounded to 2^-24 of its size, which the exponential turns into that much times the size;
+    # a few roundings follow
+    top = logits.double()[torch.isfinite(logits)].abs().max().item() / abs(temp) if torch.isfinite(logits).any() else 0.0
+    np.testing.assert_allclose(w.cpu().numpy(), want, rtol=(4 * top + 32) * 2.0 ** -24, atol=1e-30)
+
+
+@gpu
+@pytest.mark.parametrize("E,groups,kept,k", [(256, 8, 4, 8), (384, 8, 3, 6), (160, 8, 3, 6), (64, 4, 1, 8), (48, 3, 2, 4), (60, 5, 5, 7), (16, 1, 1, 2),
+                                             (32, 32, 9, 8), (1020, 17, 4, 8), (1024, 32, 5, 8), (1024, 2, 1, 3), (8, 8, 1, 1), (200, 25, 11, 8)])
+@pytest.mark.parametrize("score,group_score,with_bias", [("sigmoid", "top2", True), ("softmax", "max", False), ("sqrtsoftplus", "top2", False),
+                                                         ("softmax", "top2", True)])
+def test_route_groups(E, groups, kept, k, score, group_score, with_bias):
+    g = gen(E * 7 + groups)
+    logits = torch.randn(37, E, generator=g, device=DEV) * 2
+    bias = torch.randn(E, generator=g, device=DEV) * 0.1 if with_bias else None
+    check_route(logits, k, 2.5, True, score, bias, 1.0, groups, kept, group_score)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("T", [1, 2, 5, 130])
+def test_route_groups_types_strides_and_options(T, dtype):
+    g = gen(T)
+    wide = torch.randn(T + 1, 300, generator=g, device=DEV).to(dtype)
+    check_route(wide[1:, 3:259], 8, groups=8, kept=4)  # rows that start anywhere, 300 apart
+    check_route(wide[:T, :256].contiguous(), 6, 1.5, False, "softmax", None, 0.7, 4, 2, "max")
+    check_route(wide[:1, :96].expand(T, 96), 3, 1.0, True, "sqrtsoftplus", None, -1.3, 6, 2, "top2")
+
+
+@gpu
+def test_route_groups_ties_go_to_the_lower_index():
+    g = gen(5)
+    check_route(torch.randint(-2, 3, (200, 128), generator=g, device=DEV).float(), 8, groups=8, kept=3)
+    check_route(torch.randint(-2, 3, (200, 128), generator=g, device=DEV).float(), 8, score="softmax", groups=16, kept=5, group_score="max")
+    check_route(torch.zeros(3, 384, device=DEV), 6, score="sqrtsoftplus", groups=8, kept=4)
+
+
+@gpu
+@pytest.mark.parametrize("score", ["sigmoid", "softmax", "sqrtsoftplus"])
+def test_route_groups_border_cases_are_decided_in_64_bits(score):
+    """Neighbouring float32 logits whose scores round to the same float32 value: large ones for the sigmoid, small
+    differences under a bias that makes the keys coarse for the others."""
+    g = gen(9)
+    step = torch.randint(0, 6, (300, 64), generator=g, device=DEV)
+    logits = (torch.full((300, 64), 9.0, device=DEV).view(torch.int32) + step.to(torch.int32)).view(torch.float32)
+    bias = torch.full((64,), 3.0, device=DEV)
+    check_route(logits, 8, score=score, groups=8, kept=2, bias=bias, group_score="top2")
+    check_route(-logits, 4, score=score, groups=4, kept=2, bias=bias, group_score="max")
+
+
+@gpu
+@pytest.mark.parametrize("score", ["sigmoid", "softmax", "sqrtsoftplus"])
+def test_route_groups_infinities_and_nan(score):
+    g = gen(11)
+    logits = torch.randn(12, 64, generator=g, device=DEV)
+    logits[0] = -torch.inf
+    logits[1, 8:] = -torch.inf       # one group left
+    logits[2, ::2] = -torch.inf
+    logits[3, 17] = torch.nan
+    logits[4] = torch.nan
+    logits[5, 3] = torch.inf
+    logits[6, :4] = torch.tensor([torch.nan, torch.inf, -torch.inf, torch.nan], device=DEV)
+    logits[7] = torch.finfo(F32).min
+    logits[8, :32] = torch.finfo(F32).max
+    w, ids = B200Ops().route(logits, 8, 1.0, score_func=score, n_groups=8, topk_groups=2)
+    for row in ids.tolist():  # whatever the logits hold: distinct ids in range, of two groups
+        assert len(set(row)) == 8 and min(row) >= 0 and max(row) < 64 and len({i // 8 for i in row}) <= 2
+    for t in (2, 9, 10, 11):
+        check_route(logits[t:t + 1], 8, score=score, groups=8, kept=2)
+    if score == "sigmoid":
+        _, want = route64(logits, 8, 1.0, True, score, None, 1.0, 8, 2, "top2")
+        assert np.array_equal(ids.cpu().numpy(), want)
+
+
+@gpu
+def test_route_groups_one_group_picks_as_the_plain_router_does():
+    logits = torch.randn(500, 384, generator=gen(3), device=DEV)
+    a, b = B200Ops().route(logits, 6, 1.0, score_func="sigmoid"), B200Ops().route(logits, 6, 1.0, score_func="sigmoid", n_groups=1)
+    assert torch.equal(a[1], b[1])
+    torch.testing.assert_close(a[0], b[0], rtol=2e-6, atol=0)
+    assert B200Ops().route(logits[:0], 6, 1.0, n_groups=8)[1].shape == (0, 6)
+
+
+@gpu
+def test_route_groups_refusals():
+    ops, logits = B200Ops(), torch.zeros(4, 64, device=DEV)
+    for bad in (dict(n_groups=7), dict(n_groups=8, topk_groups=9), dict(n_groups=8, topk_groups=0), dict(n_groups=64), dict(n_groups=0),
+                dict(n_groups=8, gate_temp=0.0)):
+        with pytest.raises(RuntimeError):
+            ops.route(logits, 4, 1.0, **bad)
+    for k in (0, 9):
+        with pytest.raises(RuntimeError):
+            ops.route(logits, k, 1.0, n_groups=8)
+    with pytest.raises(RuntimeError):
+        ops.route(logits, 5, 1.0, n_groups=16, topk_groups=1)  # four experts stay
+    with pytest.raises(ValueError):
+        ops.route(logits, 4, 1.0, n_groups=8, group_score="mean")
+    with pytest.raises(ValueError):
+        ops.route(logits, 4, 1.0, n_groups=8, bias=torch.zeros(63, device=DEV))
+    with pytest.raises(RuntimeError):
+        ops.route(torch.zeros(4, 8, 8, device=DEV), 4, 1.0, n_groups=8)
+
+
+# ------------------------------------------------------------------------------------------------- plans
+def tile_list(plan):
+    t = plan._buf.cpu().numpy()
+    n = int(t[0])
+    assert n <= plan.max_tiles
+    return t[4:4 + 2 * (n + 1)].reshape(-1, 2)
+
+
+def check_plan(plan, slots, n):
+    slots = np.asarray(slots)
+    b = np.where((slots >= 0) & (slots < n), slots, n)
+    order = np.argsort(b, kind="stable")
+    assert np.array_equal(plan.rows.cpu().numpy(), order)
+    assert np.array_equal(plan.offsets.cpu().numpy(), np.concatenate([np.searchsorted(b[order], np.arange(n + 1)), [len(b)]]))
+    tiles = tile_list(plan)
+    assert tiles[-1, 0] == len(b) and (len(b) == 0 or tiles[0, 0] == 0)
+    for (a, m), (e, _) in zip(tiles[:-1], tiles[1:]):
+        assert 0 < e - a <= plan.tile and set(b[order[a:e]].tolist()) == {n if m < 0 else int(m)}
+
+
+@gpu
+@pytest.mark.parametrize("rows,n", [(1, 1), (1, 7), (31, 3), (33, 64), (257, 1), (1000, 5), (5000, 200), (16384, 64), (16384, 1023), (16385, 9), (700, 1024),
+                                    (40000, 2000), (0, 3), (0, 1500)])
+def test_plan_of_row_slots(rows, n):
+    g = gen(rows + n)
+    slots = torch.randint(-1, n + 1, (rows,), generator=g, device=DEV)
+    check_plan(AdapterPlan(slots, n), slots.cpu(), n)
+    check_plan(AdapterPlan(slots.to(torch.int32), n), slots.cpu(), n)
+
+
+@gpu
+def test_plan_of_requests():
+    offsets, slots = [0, 3, 3, 3, 40, 41, 41], [2, 0, 1, -1, 5, 0]  # empty requests, one without adapter, one outside, rows behind
+    rows = [2] * 3 + [-1] * 37 + [5] + [-1] * 9
+    for n in (3, 1100):
+        p = AdapterPlan.from_requests(torch.tensor(offsets, device=DEV), torch.tensor(slots, device=DEV), 50, n)
+        check_plan(p, rows, n)
+    check_plan(AdapterPlan.from_requests(torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(0, dtype=torch.int32, device=DEV), 20, 2), [-1] * 20, 2)
+    g = gen(1)
+    cuts = torch.randint(0, 3000, (299,), generator=g, device=DEV).sort().values
+    offs = torch.cat([cuts.new_zeros(1), cuts, cuts.new_full((1,), 3000)]).to(torch.int32)
+    s = torch.randint(-1, 17, (300,), generator=g, device=DEV)
+    check_plan(AdapterPlan.from_requests(offs, s, 3000, 17), s.repeat_interleave(offs.diff()).cpu(), 17)
+
+
+@gpu
+@pytest.mark.parametrize("T,k,E,n", [(1, 6, 384, 3), (7, 2, 8, 1), (8, 6, 384, 2), (64, 8, 64, 12), (130, 8, 16, 4), (300, 1, 5, 2), (3000, 8, 64, 4), (0, 2, 4, 2)])
+def test_plan_of_experts(T, k, E, n):
+    g = gen(T * k + E)
+    slots = torch.randint(-1, n, (T,), generator=g, device=DEV)
+    ids = torch.randint(0, E, (T, k), generator=g, device=DEV)
+    if T > 10:
+        ids[3, 0], ids[5, 1 % k] = -1, E
+    plan = AdapterPlan(slots, n)
+    s, flat = slots.cpu().numpy(), ids.cpu().numpy().reshape(-1)
+    b = np.where(s < 0, n, s).repeat(k)
+    keep = np.flatnonzero((flat >= 0) & (flat < E))
+    order = keep[np.lexsort((keep, b[keep], flat[keep]))]
+    for given in (ids, ids.to(torch.int32)):
+        p = plan.for_experts(given, E)
+        got = p.order.cpu().numpy()
+        assert np.array_equal(got[:len(order)], order) and (got[len(order):] == -1).all()
+        assert np.array_equal(p.offsets.cpu().numpy(), np.searchsorted(flat[order], np.arange(E + 1)))
+        tiles = tile_list(p)
+        assert tiles[-1, 0] == len(order) and (len(order) == 0 or tiles[0, 0] == 0)
+        for (a, m), (e, _) in zip(tiles[:-1], tiles[1:]):
+            pairs = order[a:e]
+            assert 0 < e - a <= p.tile and {(int(b[i]), int(flat[i])) for i in pairs} == ({(m // E, m % E)} if m >= 0 else {(n, int(flat[pairs[0]]))})
+
+
+def test_plans_and_adapters_refuse_without_a_gpu_or_with_bad_arguments():
+    with pytest.raises((RuntimeError, ValueError)):
+        AdapterPlan(torch.zeros(4, dtype=torch.int32), 2)  # CPU tensors
+    with pytest.raises(ValueError):
+        AdapterPlan.from_requests(torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), 4, 2)
+    for bad in (dict(dtype=F32), dict(parts=3), dict(N=65, parts=2), dict(rank=129), dict(rank=65, parts=2), dict(rank=0), dict(K=0), dict(n_adapters=0),
+                dict(experts=0)):
+        with pytest.raises(RuntimeError):
+            LowRankAdapters(**{**dict(n_adapters=2, K=64, N=64, rank=8), **bad})
+    with pytest.raises(RuntimeError):
+        LowRankAdapters(2, 64, 64, 8, device="cpu")
+
+
+def test_layer_options_are_checked():
+    z = torch.zeros(1)
+    w = ExpertWeights([z], [z], [z], [z], 64, 64, 128, "tq2")
+    for bad in (dict(n_groups=4, topk_groups=5), dict(topk_groups=2), dict(n_groups=64), dict(n_groups=4, group_score="mean"),
+                dict(n_groups=4, topk_groups=0), dict(n_groups=2, flavour="standard")):
+        with pytest.raises(ValueError):
+            MoELayer(w, 2, **bad)
+    layer = MoELayer(w, 2, n_groups=4, topk_groups=2)
+    with pytest.raises(ValueError):
+        layer.forward_routed(torch.zeros(3, 64), torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.int32), adapters=object())
+    term = tops.PackedTerm(torch.zeros(4, 16, dtype=torch.uint8), torch.ones(4, 1).half())
+    with pytest.raises(RuntimeError):
+        tops.TernaryLinear([term], 64, "tq2", 64)(torch.zeros(2, 64), adapters=object(), plan=object())
+
+
+def test_abi_argument_checks():
+    _lib.build()
+    lib = _lib.load()
+
+    def route(**kw):
+        a = {**dict(logits=0x1000, dtype=0, stride=64, T=4, E=64, groups=8, kept=4, how=1, k=4, score=0, temp=1.0, out=0x1000), **kw}
+        return lib.dst_route_group_topk(a["logits"], a["dtype"], a["stride"], None, a["T"], a["E"], a["groups"], a["kept"], a["how"], a["k"], a["score"],
+                                        a["temp"], 1, 1.0, a["out"], a["out"], None)
+
+    assert route(T=0) == _lib.OK
+    for kw, want in ((dict(logits=None), 1), (dict(out=None), 1), (dict(dtype=3), 1), (dict(score=3), 1), (dict(how=2), 1), (dict(temp=0.0), 1),
+                     (dict(temp=float("nan")), 1), (dict(k=0), 1), (dict(groups=0), 1), (dict(kept=0), 1), (dict(E=0), 1), (dict(T=-1), 1),
+                     (dict(stride=63), 2), (dict(groups=7), 2), (dict(kept=9), 2), (dict(E=1032, stride=1032), 4), (dict(groups=64), 4), (dict(k=9), 4),
+                     (dict(groups=32, kept=1), 4)):
+        assert route(**kw) == want, kw
+    p = 0x1000
+    assert lib.dst_adapter_plan(None, p, 4, 4, 0, 16, p, p, p, p, None, 0, None) == 1
+    assert lib.dst_adapter_plan(None, p, 4, 4, 4096, 16, p, p, p, p, None, 0, None) == 2
+    assert lib.dst_adapter_plan(None, p, 4, 4, 3, 0, p, p, p, p, None, 0, None) == 1
+    assert lib.dst_adapter_plan(None, None, 4, 4, 3, 16, p, p, p, p, None, 0, None) == 1
+    assert lib.dst_adapter_plan(None, p, 4, 4, 3, 16, None, p, p, p, None, 0, None) == 1
+    assert lib.dst_adapter_plan(None, p, 4, 4, 3, 16, p, p, p, p + 4, None, 0, None) == 5
+    assert lib.dst_adapter_plan(None, p, 20000, 20000, 3, 16, p, p, p, p, None, 0, None) == 1  # no workspace
+    assert lib.dst_adapter_plan_experts(p, 4, 2, 5000, p, p, 3, 16, p, p, p, p, p, 1 << 20, None) == 2
+    assert lib.dst_adapter_plan_experts(p, 4, 2, 8, p, p, 3, 16, p, p, p, p, p, 8, None) == 1
+    assert lib.dst_adapter_plan_experts(p, 1 << 30, 8, 8, p, p, 3, 16, p, p, p, p, p, 1 << 20, None) == 2
+
+    def apply(w=None, plan=None, x=p, xs=64, base=p, bt=0, bs=64, out=p, ot=1, os_=64):
+        wc = _lib.AdaptersC(**{**dict(a=p, b=p, scale=p, matrices_per_slot=1, K=64, ranks=p, K_padded=64, N=64, rank_padded=16, parts=1, dtype=0), **(w or {})})
+        pc = _lib.AdapterRowsC(**{**dict(rows=p, x_rows=p, tiles=p, max_tiles=4, tile=16), **(plan or {})})
+        import ctypes
+        return lib.dst_adapter_apply(ctypes.byref(wc), ctypes.byref(pc), x, xs, base, bt, bs, out, ot, os_, None)
+
+    assert apply(plan=dict(max_tiles=0)) == _lib.OK
+    for kw, want in ((dict(w=dict(a=None)), 1), (dict(w=dict(ranks=None)), 1), (dict(w=dict(dtype=2)), 1), (dict(w=dict(K=0)), 1), (dict(bt=3), 1), (dict(ot=-1), 1),
+                     (dict(x=None), 1), (dict(out=None), 1), (dict(w=dict(parts=3)), 2), (dict(w=dict(K_padded=32)), 2), (dict(w=dict(K_padded=72)), 2),
+                     (dict(xs=63), 2), (dict(bs=63), 2), (dict(os_=63), 2), (dict(w=dict(a=p + 2)), 5), (dict(plan=dict(tiles=p + 4)), 5),
+                     (dict(w=dict(rank_padded=24)), 4), (dict(w=dict(rank_padded=128, parts=2)), 4)):
+        assert apply(**kw) == want, kw
+
+
+# ------------------------------------------------------------------------------------------------- adapters of a projection
+def make(n, K, N, r, dtype, seed, experts=None, parts=1, rank=None):
+    g = gen(seed)
+    lead = (n,) if experts is None else (n, experts)
+    A = (torch.randn(*lead, parts * r, K, generator=g, device=DEV) / K ** 0.5).to(dtype)
+    B = (torch.randn(*lead, N, r, generator=g, device=DEV) * 0.3 / r ** 0.5).to(dtype)
+    scale = [0.5 + 0.25 * i for i in range(n)]
+    ad = LowRankAdapters(n, K, N, rank or r, dtype=dtype, experts=experts, parts=parts)
+    for i in range(n):
+        ad.load(i, A[i], B[i], scale[i])
+    return A, B, scale, ad
+
+
+def product64(x, A, B, scale, parts=1):
+    """(scale B A x, scale |B| |A| |x|) of rows x in 64 bits."""
+    x, r, n = x.double(), B.size(-1), B.size(0) // parts
+    d, S = [], []
+    for p in range(parts):
+        a, b = A[p * r:(p + 1) * r].double(), B[p * n:(p + 1) * n].double()
+        d.append(scale * (x @ a.T) @ b.T)
+        S.append(scale * (x.abs() @ a.abs().T) @ b.abs().T)
+    return torch.cat(d, -1), torch.cat(S, -1)
+
+
+def within(out, want, S, K, r, dtype):
+    tol = (K / 16 + 64 + r) * 2.0 ** -22 + (2.0 ** -17 if out.dtype != F32 and dtype == BF16 else 2.0 ** -22)
+    bound = (torch.finfo(out.dtype).eps / 2 * (1 + 2 ** -7) + 2.0 ** -23) * want.abs() + tol * S * (1 + 2 ** -7) + torch.finfo(out.dtype).tiny
+    off = (out.double() - want).abs()
+    assert bool((off <= bound).all()), float((off / bound).max())
+
+
+def check_linear(x, slots, A, B, scale, ad, base, out_dtype=None, **kw):
+    n = ad.n_adapters
+    y = ad(x, AdapterPlan(slots, n), base=base, out_dtype=out_dtype, **kw)
+    want = base.double() if base is not None else torch.zeros(x.size(0), ad.N, dtype=torch.float64, device=DEV)
+    want = want.clone()
+    S = torch.zeros_like(want)
+    for a in range(n):
+        at = slots == a
+        if at.any():
+            d, s = product64(x[at], A[a], B[a], scale[a], ad.parts)
+            want[at] += d
+            S[at] = s
+    within(y, want, S, ad.K, B.size(-1), x.dtype)
+    return y
+
+
+@gpu
+@pytest.mark.parametrize("dtype,base,out", [(BF16, F32, BF16), (BF16, F32, F32), (BF16, BF16, BF16), (F16, F32, F16), (F16, F16, F16), (F16, F32, F32),
+                                            (BF16, None, None), (BF16, F16, F32)])
+@pytest.mark.parametrize("rows,n,r", [(1, 1, 16), (5, 3, 4), (17, 2, 8), (40, 9, 32), (150, 4, 64), (333, 3, 128), (70, 2, 100)])
+def test_adapters(rows, n, r, dtype, base, out):
+    K, N = 256, 320
+    A, B, scale, ad = make(n, K, N, r, dtype, rows)
+    g = gen(rows + 1)
+    x = torch.randn(rows, K, generator=g, device=DEV).to(dtype)
+    slots = torch.randint(-1, n, (rows,), generator=g, device=DEV)
+    b = torch.randn(rows, N, generator=g, device=DEV).to(base) if base else None
+    y = check_linear(x, slots, A, B, scale, ad, b, out)
+    assert y.dtype == (out or base or dtype)
+    if b is not None:
+        none = slots < 0
+        assert torch.equal(y[none], b[none].to(y.dtype))  # rows without an adapter: the base alone, rounded
+
+
+@gpu
+@pytest.mark.parametrize("K,N", [(1, 1), (7, 3), (33, 31), (40, 8), (64, 33), (129, 200), (1000, 72), (32, 1000), (2049, 513)])
+@pytest.mark.parametrize("rows", [1, 19])
+def test_adapters_of_odd_sizes(rows, K, N):
+    for dtype, out, r in ((BF16, BF16, 5), (F16, F32, 20)):
+        A, B, scale, ad = make(2, K, N, r, dtype, K + N)
+        g = gen(K)
+        x = torch.randn(rows, K, generator=g, device=DEV).to(dtype)
+        check_linear(x, torch.randint(-1, 2, (rows,), generator=g, device=DEV), A, B, scale, ad, torch.randn(rows, N, generator=g, device=DEV), out)
+
+
+@gpu
+@pytest.mark.parametrize("parts,N,r", [(2, 128, 8), (2, 66, 16), (2, 6, 3), (2, 640, 64), (2, 200, 32)])
+def test_adapters_of_two_parts(parts, N, r):
+    A, B, scale, ad = make(3, 96, N, r, BF16, N, parts=parts)
+    g = gen(N)
+    x = torch.randn(50, 96, generator=g, device=DEV).to(BF16)
+    check_linear(x, torch.randint(-1, 3, (50,), generator=g, device=DEV), A, B, scale, ad, torch.randn(50, N, generator=g, device=DEV), BF16)
+
+
+@gpu
+@pytest.mark.parametrize("rows,K,N,r", [(2000, 512, 256, 16), (1300, 1024, 96, 64), (700, 320, 1056, 128), (4097, 64, 64, 8)])
+def test_adapters_of_long_prompts(rows, K, N, r):
+    A, B, scale, ad = make(3, K, N, r, BF16, rows)
+    g = gen(rows)
+    x = torch.randn(rows, K, generator=g, device=DEV).to(BF16)
+    slots = torch.tensor([1, -1, 0, 1, 2], device=DEV)[torch.arange(rows, device=DEV) * 5 // rows]
+    check_linear(x, slots, A, B, scale, ad, torch.randn(rows, N, generator=g, device=DEV), BF16)
+    check_linear(x, slots, A, B, scale, ad, torch.randn(rows, N, generator=g, device=DEV), F32)
+
+
+@gpu
+def test_adapters_strides_in_place_and_smaller_ranks():
+    K, N = 192, 160
+    A, B, scale, ad = make(2, K, N, 8, BF16, 1, rank=32)  # slots of rank 8 in a stack of rank 32
+    g = gen(2)
+    slots = torch.randint(-1, 2, (45,), generator=g, device=DEV)
+    for off in (0, 8, 3):  # aligned, aligned within the row, odd
+        x = torch.randn(45, K + 24, generator=g, device=DEV).to(BF16)[:, off:off + K]
+        base = torch.randn(45, N + 16, generator=g, device=DEV)[:, off:off + N]
+        y = check_linear(x, slots, A, B, scale, ad, base, BF16)
+        out = torch.full((45, N + 40), 7.0, dtype=BF16, device=DEV)
+        ad(x, AdapterPlan(slots, 2), base=base, out=out[:, off:off + N])
+        assert torch.equal(out[:, off:off + N], y) and bool((out[:, off + N:] == 7).all()) and bool((out[:, :off] == 7).all())
+    xt = torch.randn(K, 45, generator=g, device=DEV).to(BF16).T  # columns one behind the other: copied
+    b = torch.randn(45, N, generator=g, device=DEV)
+    assert torch.equal(ad(xt, AdapterPlan(slots, 2), base=b), ad(xt.contiguous(), AdapterPlan(slots, 2), base=b))
+    keep = b.clone()
+    y = ad(xt, AdapterPlan(slots, 2), base=b)
+    assert ad(xt, AdapterPlan(slots, 2), base=b, out=b) is b and torch.equal(b, y)
+    assert torch.equal(b[slots < 0], keep[slots < 0])
+
+
+@gpu
+def test_adapter_rows_do_not_depend_on_their_batch():
+    """A row's result is the same whatever shares its batch or tile, from call to call."""
+    A, B, scale, ad = make(3, 512, 256, 16, BF16, 4)
+    g = gen(4)
+    x = torch.randn(60, 512, generator=g, device=DEV).to(BF16)
+    base = torch.randn(60, 256, generator=g, device=DEV)
+    slots = torch.randint(0, 3, (60,), generator=g, device=DEV)
+    y = ad(x, AdapterPlan(slots, 3), base=base)
+    for r in (0, 17, 59):
+        assert torch.equal(ad(x[r:r + 1], AdapterPlan(slots[r:r + 1], 3), base=base[r:r + 1]), y[r:r + 1])
+    assert torch.equal(ad(x, AdapterPlan(slots, 3), base=base), y)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_adapters_with_infinities_and_nan(dtype):
+    """What is not finite stays in its row; large finite values keep their accuracy."""
+    A, B, scale, ad = make(2, 64, 64, 4, dtype, 6)
+    g = gen(6)
+    x = torch.randn(20, 64, generator=g, device=DEV).to(dtype)
+    slots = torch.zeros(20, dtype=torch.int64, device=DEV)
+    slots[10:] = -1
+    base = torch.randn(20, 64, generator=g, device=DEV)
+    clean = ad(x, AdapterPlan(slots, 2), base=base)
+    x[3, 5], x[4, 0], x[15, 2] = torch.nan, torch.inf, torch.nan
+    base[6, 1], base[16, 1] = torch.inf, torch.nan
+    y = ad(x, AdapterPlan(slots, 2), base=base)
+    hurt = torch.tensor([3, 4, 6, 16], device=DEV)
+    rest = torch.ones(20, dtype=torch.bool, device=DEV)
+    rest[hurt] = False
+    assert torch.equal(y[rest], clean[rest])
+    assert bool(y[3].isnan().all()) and not bool(y[4].isfinite().any())
+    assert y[6, 1] == torch.inf and y[16, 1].isnan() and bool(y[6, 2:].isfinite().all())
+    big = (torch.randn(4, 64, generator=g, device=DEV) * (3e4 if dtype == F16 else 1e30)).clamp(-6e4 if dtype == F16 else -1e38, 6e4 if dtype == F16 else 1e38).to(dtype)
+    A2 = (A * 64).to(dtype)
+    ad.load(1, A2[1], B[1], 1.0)
+    d, S = product64(big, A2[1], B[1], 1.0)
+    within(ad(big, AdapterPlan(torch.ones(4, dtype=torch.int32, device=DEV), 2), out_dtype=F32), d, S, 64, 4, dtype)
+    ad.load(0, torch.ones(1, 64, dtype=dtype, device=DEV), torch.ones(64, 1, dtype=dtype, device=DEV))
+    same = ad(torch.full((1, 64), torch.inf, dtype=dtype, device=DEV), AdapterPlan(torch.zeros(1, dtype=torch.int32, device=DEV), 2))
+    assert bool((same == torch.inf).all())
+
+
+@gpu
+def test_empty_slots_and_reloading():
+    A, B, scale, ad = make(2, 128, 64, 16, BF16, 8)
+    x = torch.randn(9, 128, generator=gen(8), device=DEV).to(BF16)
+    base = torch.randn(9, 64, generator=gen(9), device=DEV)
+    plan = AdapterPlan(torch.ones(9, dtype=torch.int32, device=DEV), 2)
+    y = ad(x, plan, base=base)
+    ad.clear(1)
+    assert torch.equal(ad(x, plan, base=base), base)
+    ad.load(1, A[1], B[1], scale[1])
+    assert torch.equal(ad(x, plan, base=base), y)
+    with pytest.raises(IndexError):
+        ad.load(2, A[1], B[1])
+    with pytest.raises(IndexError):
+        ad.clear(-1)
+    assert ad(x[:0], AdapterPlan(torch.zeros(0, dtype=torch.int32, device=DEV), 2), base=base[:0]).shape == (0, 64)
+
+
+@gpu
+def test_adapter_refusals():
+    A, B, scale, ad = make(2, 128, 64, 16, BF16, 8)
+    x, base = torch.zeros(9, 128, dtype=BF16, device=DEV), torch.zeros(9, 64, device=DEV)
+    slots = torch.zeros(9, dtype=torch.int32, device=DEV)
+    plan = AdapterPlan(slots, 2)
+    for kw in (dict(x=x[:8]), dict(x=x[:, :64]), dict(base=base[:8]), dict(base=base.double()), dict(plan=AdapterPlan(slots, 3)),
+               dict(plan=plan.for_experts(slots[:, None], 2)), dict(out=torch.zeros(9, 63, device=DEV)), dict(out=torch.zeros(64, 9, device=DEV).T),
+               dict(out=base, out_dtype=BF16), dict(pair_rows=True), dict(x=x.cpu())):
+        args = {**dict(x=x, plan=plan, base=base), **kw}
+        with pytest.raises(RuntimeError):
+            ad(args.pop("x"), args.pop("plan"), **args)
+    with pytest.raises(TypeError):
+        ad(x.half(), plan, base=base)
+    for bad in ((A[0][:, :64], B[0]), (A[0], B[0][:32]), (A[0][:8], B[0]), (torch.zeros(32, 128), torch.zeros(64, 32))):
+        with pytest.raises(RuntimeError):
+            ad.load(0, *bad)
+    with pytest.raises(RuntimeError):
+        AdapterPlan(slots.float(), 2)
+    with pytest.raises(RuntimeError):
+        AdapterPlan(slots, 0)
+    with pytest.raises(RuntimeError):
+        plan.for_experts(slots[:8, None], 2)
+
+
+# ------------------------------------------------------------------------------------------------- adapters of experts
+@gpu
+@pytest.mark.parametrize("T,k,E,n,K,N,r,parts", [(1, 4, 16, 2, 128, 256, 16, 2), (9, 3, 8, 3, 256, 128, 8, 1), (200, 4, 8, 2, 64, 96, 32, 2),
+                                                 (600, 2, 4, 3, 96, 72, 16, 1), (33, 2, 6, 2, 50, 34, 4, 2)])
+@pytest.mark.parametrize("pair_rows", [False, True])
+def test_adapters_of_experts(T, k, E, n, K, N, r, parts, pair_rows):
+    A, B, scale, ad = make(n, K, N, r, BF16, T, experts=E, parts=parts)
+    g = gen(T)
+    slots = torch.randint(-1, n, (T,), generator=g, device=DEV)
+    ids = torch.rand(T, E, generator=g, device=DEV).topk(k, -1).indices.to(torch.int32)
+    if T > 50:
+        ids[7, 0] = E  # dropped
+    pairs = AdapterPlan(slots, n).for_experts(ids, E)
+    P, V = T * k, int(pairs.offsets[-1])
+    x = torch.randn(P if pair_rows else T, K, generator=g, device=DEV).to(BF16)
+    base = torch.randn(P, N, generator=g, device=DEV)
+    out = torch.full((P, N), 7.0, dtype=BF16, device=DEV)
+    ad(x, pairs, base=base, out=out, pair_rows=pair_rows)
+    want, S = base.double().clone(), torch.zeros(P, N, dtype=torch.float64, device=DEV)
+    order = pairs.order.tolist()
+    for p in range(V):
+        t, e = order[p] // k, int(ids.view(-1)[order[p]])
+        a = int(slots[t])
+        if a >= 0:
+            d, s = product64(x[p:p + 1] if pair_rows else x[t:t + 1], A[a, e], B[a, e], scale[a], parts)
+            want[p] += d[0]
+            S[p] += s[0]
+    within(out[:V], want[:V], S[:V], K, r, BF16)
+    assert bool((out[V:] == 7).all())  # positions behind the last pair are left as they were
+
+
+# ------------------------------------------------------------------------------------------------- together
+def ternary(rows, K, fmt, g):
+    t = torch.randint(-1, 2, (rows, K), generator=g, device=DEV, dtype=torch.int8)
+    s = (torch.randn(rows, K // 128, generator=g, device=DEV) * 0.3 - 3).exp().half()
+    return pack(t, fmt), s, t.double() * s.double().repeat_interleave(128, 1)
+
+
+@gpu
+@pytest.mark.parametrize("act,fmt,rows", [("bf16", "tq2", 3), ("bf16", "tq1", 100), ("int8", "tq2", 40)])
+def test_ternary_linear_with_adapters(act, fmt, rows):
+    g = gen(rows)
+    K, N = 512, 256
+    p, s, W = ternary(N, K, fmt, g)
+    lin = tops.TernaryLinear([tops.PackedTerm(p, s)], K, fmt, 128, act=act)
+    A, B, scale, ad = make(3, K, N, 8, BF16, rows)
+    x = torch.randn(rows, K, generator=g, device=DEV).to(BF16)
+    slots = torch.randint(-1, 3, (rows,), generator=g, device=DEV)
+    plan = AdapterPlan(slots, 3)
+    y = lin(x, adapters=ad, plan=plan)
+    assert y.dtype == BF16 and torch.equal(y, ad(x, plan, base=lin(x, F32), out_dtype=BF16))
+    assert torch.equal(lin(x.view(1, rows, K), adapters=ad, plan=plan)[0], y)
+    assert torch.equal(lin(x, F32, adapters=ad, plan=plan)[slots < 0], lin(x, F32)[slots < 0])
+    want = x.double() @ W.T
+    for a in range(3):
+        want[slots == a] += product64(x[slots == a], A[a], B[a], scale[a])[0]
+    # the projection alone is within 2e-3 of its norm (int8 activations: 1 / 254 of a row's largest value each, 2e-2), bf16 2^-9
+    assert float((y.double() - want).norm() / want.norm()) <= (2e-2 if act == "int8" else 2e-3 + 2.0 ** -8)
+    with pytest.raises(ValueError):
+        lin(x, adapters=ad)
+    with pytest.raises(RuntimeError):
+        lin(x, adapters=make(3, K, N + 32, 8, BF16, 1)[3], plan=plan)
+
+
+def layer_of(E, H, I, fmt, g, top_k=2, **kw):
+    w13, s13, W13 = zip(*(ternary(2 * I, H, fmt, g) for _ in range(E)))
+    w2, s2, W2 = zip(*(ternary(H, I, fmt, g) for _ in range(E)))
+    ew = ExpertWeights([torch.stack(w13)], [torch.stack(s13)], [torch.stack(w2)], [torch.stack(s2)], H, I, 128, fmt).prepare()
+    return MoELayer(ew, top_k, **kw), W13, W2
+
+
+def adapted64(x, weights, ids, slots, W13, W2, gu_ad, down_ad, I, rounded):
+    """The V4 layer in 64 bits from its routing; `rounded`: with the layer's own roundings to bf16."""
+    cut = (lambda v: v.to(BF16).double()) if rounded else (lambda v: v)
+    y = torch.zeros_like(x, dtype=torch.float64)
+    (A13, B13, scale), (A2, B2, _) = gu_ad, down_ad
+    for t in range(x.size(0)):
+        for j in range(ids.size(1)):
+            e, a, v = int(ids[t, j]), int(slots[t]), x[t:t + 1].double()
+            gu = v @ W13[e].T
+            if a >= 0:
+                gu = gu + product64(v, A13[a, e], B13[a, e], scale[a], 2)[0]
+            gu = cut(gu)
+            gate, up = gu[:, :I], gu[:, I:]
+            h = cut(float(weights[t, j]) * gate * torch.sigmoid(gate) * up)
+            d = h @ W2[e].T
+            if a >= 0:
+                d = d + product64(h, A2[a, e], B2[a, e], scale[a])[0]
+            y[t] += cut(d)[0]
+    return cut(y)
+
+
+@gpu
+@pytest.mark.parametrize("T,fmt", [(3, "tq2"), (60, "tq1")])
+def test_adapted_layer_routed_in_groups(T, fmt):
+    """Router in groups -> plan of the pairs -> expert products with adapters -> combine, against 64 bits: no further off than
+    the layer's own roundings take it, with a quarter to spare (as the layer without adapters is held to)."""
+    E, H, I, n, r = 8, 256, 128, 3, 8
+    g = gen(T)
+    layer, W13, W2 = layer_of(E, H, I, fmt, g, n_groups=4, topk_groups=2, score_func="sigmoid", route_scale=1.5,
+                              gate_bias=torch.randn(E, generator=g, device=DEV) * 0.1)
+    ad = ExpertAdapters(n, E, H, I, r)
+    A13, B13, scale, _ = make(n, H, 2 * I, r, BF16, 1, experts=E, parts=2)
+    A2, B2, _, _ = make(n, I, H, r, BF16, 2, experts=E)
+    for a in range(n):
+        ad.load(a, (A13[a, :, :r], B13[a, :, :I]), (A13[a, :, r:], B13[a, :, I:]), (A2[a], B2[a]), scale[a])
+    x = torch.randn(T, H, generator=g, device=DEV).to(BF16)
+    logits = torch.randn(T, E, generator=g, device=DEV)
+    slots = torch.randint(-1, n, (T,), generator=g, device=DEV)
+    plan = AdapterPlan(slots, n)
+    y = layer(x, logits, adapters=ad, plan=plan)
+    weights, ids = layer.route(logits)
+    assert len({int(i) // 2 for i in ids[0]}) <= 2
+    exact = adapted64(x, weights, ids, slots, W13, W2, (A13, B13, scale), (A2, B2, scale), I, False)
+    ref = adapted64(x, weights, ids, slots, W13, W2, (A13, B13, scale), (A2, B2, scale), I, True)
+    e_ref, e_got = ((v.double() - exact).norm() / exact.norm() for v in (ref, y))
+    assert float(e_got) <= max(1.25 * float(e_ref), 2e-3), (float(e_got), float(e_ref))
+    bare = layer(x, logits)
+    assert float((y.double() - bare.double()).norm() / bare.double().norm()) > 0.02  # the adapters do something
+    assert torch.equal(layer.forward_routed(x, weights, ids.long(), ad, plan), y)
+    assert torch.equal(y[slots < 0], layer(x, logits, adapters=ad, plan=AdapterPlan(torch.full_like(slots, -1), n))[slots < 0])
+    with pytest.raises(ValueError):
+        layer(x, logits, adapters=ad)
+
+
+@gpu
+def test_adapted_standard_layer_and_dropped_ids():
+    E, H, I, T = 4, 256, 128, 20
+    g = gen(3)
+    layer, _, _ = layer_of(E, H, I, "tq2", g, flavour="standard")
+    ad = ExpertAdapters(1, E, H, I, 4)  # an empty slot: what the layer does without adapters, but for the order of its rows
+    x = torch.randn(T, H, generator=g, device=DEV).to(BF16)
+    logits = torch.randn(T, E, generator=g, device=DEV)
+    plan = AdapterPlan(torch.zeros(T, dtype=torch.int32, device=DEV), 1)
+    torch.testing.assert_close(layer(x, logits, adapters=ad, plan=plan).float(), layer(x, logits).float(), rtol=2 ** -6, atol=2 ** -6)
+    v4, _, _ = layer_of(E, H, I, "tq2", g)
+    weights, ids = v4.route(logits)
+    ids[2, 1], ids[5, 0] = -1, E
+    torch.testing.assert_close(v4.forward_routed(x, weights, ids, ad, plan).float(), v4.forward_routed(x, weights, ids).float(), rtol=2 ** -6, atol=2 ** -6)
+
+
+@gpu
+def test_captured_steps_follow_their_inputs():
+    """Router, plan and adapters in one captured graph: replayed on other logits, rows and requests, another adapter loaded."""
+    E, n, K, N, T = 64, 4, 256, 128, 48
+    A, B, scale, ad = make(n, K, N, 16, BF16, 2)
+    g = gen(12)
+    x, base = torch.randn(T, K, generator=g, device=DEV).to(BF16), torch.randn(T, N, generator=g, device=DEV)
+    logits = torch.randn(T, E, generator=g, device=DEV)
+    offsets = torch.tensor([0, 10, 30, 48], dtype=torch.int32, device=DEV)
+    slots = torch.tensor([0, 2, -1], dtype=torch.int32, device=DEV)
+
+    def step():
+        p = AdapterPlan.from_requests(offsets, slots, T, n)
+        w, ids = B200Ops().route(logits, 4, 1.0, score_func="sigmoid", n_groups=8, topk_groups=3)
+        pairs = p.for_experts(ids, E)
+        return ad(x, p, base=base, out_dtype=BF16), w, ids, pairs.order, pairs.offsets
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        eager = step()  # on a stream of its own
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = step()
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, eager))
+    for turn in range(3):
+        x.copy_(torch.randn(T, K, generator=g, device=DEV).to(BF16))
+        logits.copy_(torch.randn(T, E, generator=g, device=DEV))
+        offsets.copy_(torch.tensor([[0, 1, 2, 48], [0, 0, 48, 48], [0, 5, 9, 20]][turn], dtype=torch.int32))
+        slots.copy_(torch.tensor([[3, 1, 0], [1, 1, 1], [2, 7, 0]][turn], dtype=torch.int32))
+        ad.load(1, A[turn], B[turn], 0.5 + turn)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+@gpu
+def test_two_streams_at_once():
+    A, B, scale, ad = make(4, 1024, 512, 32, BF16, 2)
+    g = gen(13)
+    xs = [torch.randn(300, 1024, generator=g, device=DEV).to(BF16) for _ in range(2)]
+    bases = [torch.randn(300, 512, generator=g, device=DEV) for _ in range(2)]
+    plans = [AdapterPlan(torch.randint(-1, 4, (300,), generator=g, device=DEV), 4) for _ in range(2)]
+    want = [ad(x, p, base=b) for x, p, b in zip(xs, plans, bases)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ad(xs[i], plans[i], base=bases[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
