@@ -7,16 +7,34 @@
 //   picks                        the top_k largest keys among the kept groups' experts (equal keys: the lower id), in that order
 //   weight_i = s of pick i, divided by the picks' sum + 1e-20 when renormalised (top_k > 1), times route_scale
 //
-// The picks are those of exact arithmetic: keys closer than the rounding of their scores are compared in 64 bits. A NaN ranks
-// above every number, so a token's ids are distinct and inside [0, E) whatever the logits hold.
-#include <type_traits>
-
+// The picks are those of exact arithmetic. Without a bias f keeps the order of the logits, which decide by themselves; sums of two
+// scores and keys with a bias are compared in float32 where they are further apart than their rounding errors can reach, and a
+// token with a closer border is done again in 64 bits. A NaN ranks above every number (such a token goes the 64-bit way too), so
+// a token's ids are distinct and inside [0, E) whatever the logits hold.
 #include "dst_common.cuh"
 
 namespace dst {
 namespace {
 
-// A key as an unsigned number of the same order; NaNs above everything and equal among themselves, 0 below every key.
+struct GroupRoute {
+  const void* logits;
+  int64_t stride;
+  const float* bias;
+  int64_t T;
+  int dtype, E, groups, size, kept, two, top_k, renorm;
+  int shift, chunk, stride_s;  // 1 << shift lanes for a group, experts of a lane, and the words between lanes in shared memory
+  int vec;                     // rows of float32 logits can be copied 16 bytes at a time, a lane's are whole pieces
+  int vec_bias;                // so can a lane's biases
+  uint32_t per_lane;           // 2^32 / (chunk / 4), rounded up: a division of piece numbers
+  float temp, scale;
+  float* weights;
+  int32_t* ids;
+};
+
+constexpr int WARPS = 4, TOP = 8;  // TOP: picks of a token at most
+constexpr unsigned FULL = 0xffffffffu;
+
+// A number as an unsigned one of the same order; NaNs above everything and equal among themselves, 0 below every number.
 __device__ __forceinline__ uint64_t order_of(double v) {
   if (v != v) return ~0ull;
   const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
@@ -26,130 +44,457 @@ __device__ __forceinline__ double value_of(uint64_t r) {
   if (r == ~0ull) return __longlong_as_double(0x7ff8000000000000ll);
   return __longlong_as_double((long long)((r >> 63) ? (r & ~(1ull << 63)) : ~r));
 }
+__device__ __forceinline__ uint32_t order_of(float v) {  // of a number
+  const uint32_t u = __float_as_uint(v + 0.f);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t r) { return __uint_as_float(r ^ ((uint32_t)(~(int32_t)r >> 31) | 0x80000000u)); }
 
-struct GroupRoute {
-  const void* logits;
-  int64_t stride;
-  const float* bias;
-  int64_t T;
-  int E, groups, size, lanes, chunk, kept, two, top_k, score, renorm;  // lanes: of the warp for one group; chunk: experts per lane
-  float temp, scale;
-  float* weights;
-  int32_t* ids;
-};
-
-template <typename T>
-__device__ __forceinline__ float logit(const T* p) {
-  if constexpr (sizeof(T) == 4) return *p;
-  else if constexpr (std::is_same<T, __half>::value) return __half2float(*p);
-  else return __bfloat162float(*p);
+__device__ __forceinline__ float load_logit(const GroupRoute& a, int64_t i) {
+  if (a.dtype == DST_OUT_F32) return static_cast<const float*>(a.logits)[i];
+  if (a.dtype == DST_OUT_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(a.logits)[i]);
+  return __half2float(static_cast<const __half*>(a.logits)[i]);
 }
 
-__device__ __forceinline__ uint64_t shfl64(uint64_t v, int src) { return __shfl_sync(0xffffffffu, v, src); }
-__device__ __forceinline__ uint64_t shfl64_xor(uint64_t v, int m) { return __shfl_xor_sync(0xffffffffu, v, m); }
+template <int SCORE>
+__device__ __forceinline__ double score64(double z, double mx, double sum) {
+  if (SCORE == DST_SCORE_SOFTMAX) return exp(z - mx) / sum;
+  if (SCORE == DST_SCORE_SIGMOID) return 1.0 / (1.0 + exp(-z));
+  return sqrt(fmax(z, 0.0) + log1p(exp(-fabs(z))));  // a NaN comes through log1p
+}
 
-// One token by one warp in 64 bits. A group belongs to `lanes` neighbouring lanes (a power of two), a lane to `chunk`
-// consecutive experts of it, so ids rise with the lane and with j.
-template <int PL, typename T>
-__device__ __forceinline__ void route_token(const GroupRoute& a, int64_t t, int lane) {
-  const T* row = static_cast<const T*>(a.logits) + t * a.stride;
-  const int group = lane / a.lanes, first = (lane % a.lanes) * a.chunk;
-  int n = group < a.groups ? min(a.chunk, a.size - first) : 0;
-  const int id0 = group * a.size + first;
-  double s[PL];
-  double mx = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < PL; ++j) {
-    s[j] = j < n ? (double)logit(row + id0 + j) / (double)a.temp : -INFINITY;
-    mx = fmax(mx, s[j]);
+// A token in 64 bits by the whole block, its keys in shared memory (`keys` [E]).
+template <int SCORE>
+__device__ __noinline__ void route_exact(const GroupRoute& a, int64_t t, uint64_t* keys, double* red) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t row = t * a.stride;
+  const double temp = a.temp;
+  double mx = -INFINITY, sum = 0.0;
+  if (SCORE == DST_SCORE_SOFTMAX) {
+    for (int e = tid; e < a.E; e += WARPS * 32) mx = fmax(mx, (double)load_logit(a, row + e) / temp);
+    for (int off = 16; off > 0; off >>= 1) mx = fmax(mx, __shfl_xor_sync(FULL, mx, off));
+    if (lane == 0) red[warp] = mx;
+    __syncthreads();
+    for (int w = 0; w < WARPS; ++w) mx = fmax(mx, red[w]);
+    __syncthreads();
+    for (int e = tid; e < a.E; e += WARPS * 32) sum += exp((double)load_logit(a, row + e) / temp - mx);
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(FULL, sum, off);
+    if (lane == 0) red[warp] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int w = 0; w < WARPS; ++w) sum += red[w];
   }
-  if (a.score == DST_SCORE_SOFTMAX) {
-    for (int off = 16; off > 0; off >>= 1) mx = fmax(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-    double sum = 0.0;
-#pragma unroll
-    for (int j = 0; j < PL; ++j) {
-      s[j] = exp(s[j] - mx);
-      if (j < n) sum += s[j];
+  for (int e = tid; e < a.E; e += WARPS * 32) {
+    const double s = score64<SCORE>((double)load_logit(a, row + e) / temp, mx, sum);
+    keys[e] = order_of(a.bias ? s + (double)a.bias[e] : s);
+  }
+  __syncthreads();
+  if (warp == 0) {  // a group is a matter of 32 >> wide neighbouring lanes, each with its own run of experts
+    int wide = 0;
+    while ((1 << wide) < a.groups) ++wide;
+    const int lanes = 32 >> wide, group = lane / lanes, run = (a.size + lanes - 1) / lanes, first = (lane % lanes) * run;
+    const int n = group < a.groups ? min(run, a.size - first) : 0, id0 = group * a.size + first;
+    uint64_t m1 = 0, m2 = 0;
+    for (int j = 0; j < n; ++j) {
+      const uint64_t k = keys[id0 + j];
+      if (k > m1) m2 = m1, m1 = k;
+      else if (k > m2) m2 = k;
     }
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    const uint64_t own = m1;
+    for (int off = 1; off < lanes; off <<= 1) {
+      const uint64_t o1 = __shfl_xor_sync(FULL, m1, off), o2 = __shfl_xor_sync(FULL, m2, off);
+      if (o1 > m1) m2 = m1 > o2 ? m1 : o2, m1 = o1;
+      else m2 = m2 > o1 ? m2 : o1;
+    }
+    const uint64_t g = a.two && m2 ? order_of(value_of(m1) + value_of(m2)) : m1;
+    int better = 0;
+    for (int h = 0; h < a.groups; ++h) {
+      const uint64_t o = __shfl_sync(FULL, g, h * lanes);
+      better += o > g || (o == g && h < group);
+    }
+    const bool keep = group < a.groups && better < a.kept;
+    uint64_t best = keep ? own : 0;  // the lane's largest that is left
+    double my_w = 0.0, wsum = 0.0;
+    int my_id = 0;
+    for (int r = 0; r < a.top_k; ++r) {
+      uint64_t top = best;
+      for (int off = 16; off > 0; off >>= 1) {
+        const uint64_t o = __shfl_xor_sync(FULL, top, off);
+        top = o > top ? o : top;
+      }
+      const int win = __ffs(__ballot_sync(FULL, best == top)) - 1;
+      int at = 0;
+      if (lane == win) {
+        uint64_t next = 0;
+        bool taken = false;
+        for (int j = 0; j < n; ++j) {
+          const uint64_t k = keys[id0 + j];
+          if (k == best && !taken) keys[id0 + j] = 0, at = id0 + j, taken = true;
+          else if (k > next) next = k;
+        }
+        best = next;
+      }
+      at = __shfl_sync(FULL, at, win);
+      if (lane == r) my_id = at;
+    }
+    if (lane < a.top_k) my_w = score64<SCORE>((double)load_logit(a, row + my_id) / temp, mx, sum);
+    wsum = my_w;
+    for (int off = 4; off > 0; off >>= 1) wsum += __shfl_xor_sync(FULL, wsum, off);
+    if (lane < a.top_k) {
+      a.weights[t * a.top_k + lane] = (float)((a.renorm && a.top_k > 1 ? my_w / (wsum + 1e-20) : my_w) * (double)a.scale);
+      a.ids[t * a.top_k + lane] = my_id;
+    }
+  }
+  __syncthreads();
+}
+
+// float32 scores: near ones for the selection, which allows for their errors (units of 2^-24 of the score: the hardware's
+// exponential 4 and 2 |z| for its argument, reciprocal and square root 2 each), and those of the picks, for the weights.
+// log(1 + e) = 2 artanh(e / (2 + e)) = 2 (t + t^3 / 3 + t^5 / 5 + ...), t <= 1 / 3: seven terms leave 2e-8 of it.
+template <int SCORE>
+__device__ __forceinline__ float score_near(float z) {
+  if (SCORE == DST_SCORE_SIGMOID) return __fdividef(1.f, 1.f + __expf(-z));
+  const float e = __expf(-fabsf(z)), t = __fdividef(e, 2.f + e), u = t * t;
+  const float p = fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, 2.f / 13.f, 2.f / 11.f), 2.f / 9.f), 2.f / 7.f), 2.f / 5.f), 2.f / 3.f), 2.f);
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(fmaf(t, p, fmaxf(z, 0.f))));
+  return r;
+}
+template <int SCORE>
+__device__ __forceinline__ float score_of(float z) {
+  if (SCORE == DST_SCORE_SIGMOID) return 1.f / (1.f + expf(-z));
+  return sqrtf(fmaxf(z, 0.f) + log1pf(expf(-fabsf(z))));
+}
+
+__device__ __forceinline__ void swap_down(uint32_t& a, uint32_t& b) {  // a >= b afterwards
+  const uint32_t hi = max(a, b);
+  b = min(a, b);
+  a = hi;
+}
+// Eight numbers in descending order (19 exchanges)
+__device__ __forceinline__ void sort8(uint32_t (&v)[8]) {
+  swap_down(v[0], v[1]), swap_down(v[2], v[3]), swap_down(v[4], v[5]), swap_down(v[6], v[7]);
+  swap_down(v[0], v[2]), swap_down(v[1], v[3]), swap_down(v[4], v[6]), swap_down(v[5], v[7]);
+  swap_down(v[1], v[2]), swap_down(v[5], v[6]);
+  swap_down(v[0], v[4]), swap_down(v[1], v[5]), swap_down(v[2], v[6]), swap_down(v[3], v[7]);
+  swap_down(v[2], v[4]), swap_down(v[3], v[5]);
+  swap_down(v[1], v[2]), swap_down(v[3], v[4]), swap_down(v[5], v[6]);
+}
+// The eight largest of two descending lists, descending: the larger of each pair from opposite ends, a bitonic list, then sorted
+__device__ __forceinline__ void merge8(uint32_t (&v)[8], const uint32_t (&w)[8]) {
 #pragma unroll
-    for (int j = 0; j < PL; ++j) s[j] = s[j] / sum;
-  } else if (a.score == DST_SCORE_SIGMOID) {
+  for (int i = 0; i < 8; ++i) v[i] = max(v[i], w[7 - i]);
 #pragma unroll
-    for (int j = 0; j < PL; ++j) s[j] = 1.0 / (1.0 + exp(-s[j]));
+  for (int d = 4; d > 0; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (!(i & d)) swap_down(v[i], v[i | d]);
+}
+
+// LPT lanes a token (8, 16 or 32; at least one a group). A group belongs to 1 << shift neighbouring lanes, a lane to `chunk`
+// consecutive experts of it, so ids rise with the lane and inside it; the lane's numbers lie in shared memory at a stride of an odd
+// number of 16-byte pieces. A lane keeps its eight largest numbers sorted; a round takes the largest head of the token's lanes, the
+// lowest lane first. Which experts the picks were is found at the end from the numbers. Returns whether the lane's token has to be
+// done in 64 bits. The warp stays together throughout: its tokens differ in what they need.
+template <int SCORE, int LPT>
+__device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, bool valid, uint32_t* mine /* of the token */) {
+  const int lane = threadIdx.x & 31, tl = lane % LPT;
+  const unsigned segment = LPT == 32 ? FULL : ((1u << LPT) - 1u) << (lane - tl);
+  const auto seg_max = [&](uint32_t v) {
+    if (LPT == 32) return __reduce_max_sync(FULL, v);
+#pragma unroll
+    for (int off = LPT / 2; off > 0; off >>= 1) v = max(v, __shfl_xor_sync(FULL, v, off));
+    return v;
+  };
+  const auto seg_any = [&](bool v) { return (__ballot_sync(FULL, v) & segment) != 0; };
+  const int64_t row = t * a.stride;
+  const int group = tl >> a.shift, first = (tl & ((1 << a.shift) - 1)) * a.chunk;
+  const int n = group < a.groups ? min(a.chunk, a.size - first) : 0, id0 = group * a.size + first;
+  uint32_t* own = mine + tl * a.stride_s;
+  if (a.vec) {
+    const int pieces = a.E >> 2, gap = (a.stride_s - a.chunk) >> 2;  // pieces of the row, and those between two lanes'
+    const float* from = static_cast<const float*>(a.logits) + row;
+    for (int i = tl; i < pieces; i += LPT) {
+      const uint32_t to = (uint32_t)__cvta_generic_to_shared(mine + 4 * (i + gap * (int)__umulhi((uint32_t)i, a.per_lane)));
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from + 4 * i) : "memory");
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
   } else {
+    for (int j = 0; j < n; ++j) own[j] = __float_as_uint(load_logit(a, row + id0 + j));
+  }
+  // The lane's numbers in blocks of eight. A logit is negated under a negative temperature: experts rank by it as they do by their
+  // scores. zmax, zmin and `special` (a NaN from anything that is not finite) come out of the first pass.
+  const bool flip = a.temp < 0.f;
+  const float inv_temp = 1.f / fabsf(a.temp);
+  float zmax = -INFINITY, zmin = INFINITY, special = 0.f, inv_sum = 1.f, mx = 0.f;
+  const auto eight = [&](int j0, float (&z)[8]) {
+    const float4 u = *reinterpret_cast<const float4*>(own + j0), v = *reinterpret_cast<const float4*>(own + j0 + 4);
+    z[0] = u.x, z[1] = u.y, z[2] = u.z, z[3] = u.w, z[4] = v.x, z[5] = v.y, z[6] = v.z, z[7] = v.w;
+    if (j0 + 8 > n) {  // behind the last one: the first again
 #pragma unroll
-    for (int j = 0; j < PL; ++j) s[j] = sqrt(fmax(s[j], 0.0) + log1p(exp(-fabs(s[j]))));
-  }
-  uint64_t rank[PL], m1 = 0, m2 = 0;
-#pragma unroll
-  for (int j = 0; j < PL; ++j) {
-    rank[j] = j < n ? order_of(a.bias ? s[j] + (double)a.bias[id0 + j] : s[j]) : 0ull;
-    if (rank[j] > m1) m2 = m1, m1 = rank[j];
-    else if (rank[j] > m2) m2 = rank[j];
-  }
-  for (int off = 1; off < a.lanes; off <<= 1) {
-    const uint64_t o1 = shfl64_xor(m1, off), o2 = shfl64_xor(m2, off);
-    if (o1 > m1) m2 = m1 > o2 ? m1 : o2, m1 = o1;
-    else m2 = m2 > o1 ? m2 : o1;
-  }
-  uint64_t g = m1;
-  if (a.two && m2) g = order_of(value_of(m1) + value_of(m2));
-  int better = 0;
-  for (int h = 0; h < a.groups; ++h) {
-    const uint64_t o = shfl64(g, h * a.lanes);
-    better += o > g || (o == g && h < group);
-  }
-  if (better >= a.kept) {
-#pragma unroll
-    for (int j = 0; j < PL; ++j) rank[j] = 0;
-  }
-  double my_w = 0.0, wsum = 0.0;
-  int my_id = 0;
-  for (int r = 0; r < a.top_k; ++r) {
-    uint64_t best = 0;
-    int at = 0;
-    double w = 0.0;
-#pragma unroll
-    for (int j = 0; j < PL; ++j)
-      if (rank[j] > best) best = rank[j], at = j, w = s[j];
-    uint64_t top = best;
-    for (int off = 16; off > 0; off >>= 1) {
-      const uint64_t o = shfl64_xor(top, off);
-      top = o > top ? o : top;
+      for (int i = 1; i < 8; ++i)
+        if (j0 + i >= n) z[i] = z[0];
     }
-    const int win = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+    if (flip) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] = -z[i];
+    }
+  };
+  const auto range = [&](const float (&z)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      zmax = fmaxf(zmax, z[i]);
+      zmin = fminf(zmin, z[i]);
+      special = fmaf(z[i], 0.f, special);
+    }
+  };
+  if (SCORE == DST_SCORE_SOFTMAX) {
+    for (int j0 = 0; j0 < n; j0 += 8) {
+      float z[8];
+      eight(j0, z);
+      range(z);
+    }
+    mx = value_of(seg_max(order_of(zmax))) * inv_temp;
+    float sum = 0.f;
+    for (int j0 = 0; j0 < n; j0 += 8) {
+      float z[8];
+      eight(j0, z);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += j0 + i < n ? __expf(z[i] * inv_temp - mx) : 0.f;
+    }
+#pragma unroll
+    for (int off = LPT / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(FULL, sum, off);
+    inv_sum = 1.f / sum;
+  }
+  const auto near = [&](float v) { return SCORE == DST_SCORE_SOFTMAX ? __expf(v * inv_temp - mx) * inv_sum : score_near<SCORE>(v * inv_temp); };
+
+  uint32_t top[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  float special_key = 0.f;
+  for (int j0 = 0; j0 < n; j0 += 8) {
+    float z[8];
+    eight(j0, z);
+    if (SCORE != DST_SCORE_SOFTMAX) range(z);
+    if (a.bias) {
+      float b[8];
+      if (a.vec_bias) {
+        const float4 u = __ldg(reinterpret_cast<const float4*>(a.bias + id0 + j0)), v = __ldg(reinterpret_cast<const float4*>(a.bias + id0 + j0 + 4));
+        b[0] = u.x, b[1] = u.y, b[2] = u.z, b[3] = u.w, b[4] = v.x, b[5] = v.y, b[6] = v.z, b[7] = v.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = __ldg(a.bias + id0 + (j0 + i < n ? j0 + i : j0));
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        z[i] = near(z[i]) + b[i];
+        special_key = fmaf(z[i], 0.f, special_key);
+      }
+    }
+    uint32_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = order_of(z[i]);
+    if (j0 + 8 > n) {
+#pragma unroll
+      for (int i = 1; i < 8; ++i)
+        if (j0 + i >= n) v[i] = 0u;
+    }
+    *reinterpret_cast<uint4*>(own + j0) = make_uint4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<uint4*>(own + j0 + 4) = make_uint4(v[4], v[5], v[6], v[7]);
+    sort8(v);
+    if (j0 == 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top[i] = v[i];
+    } else {
+      merge8(top, v);
+    }
+  }
+  bool again = false;
+  if (__any_sync(FULL, special != 0.f || special_key != 0.f)) {  // NaNs, infinities above and NaN keys: in 64 bits
+    zmin = INFINITY;
+    for (int j = 0; j < n; ++j) {
+      const float v = load_logit(a, row + id0 + j), z = flip ? -v : v, b = a.bias ? a.bias[id0 + j] : 0.f;
+      again = again || !(z < INFINITY) || b != b;
+      zmin = fminf(zmin, z == -INFINITY ? INFINITY : z);
+    }
+    again = seg_any(again);
+  }
+  zmax = value_of(seg_max(order_of(zmax)));
+  again = again || (SCORE == DST_SCORE_SOFTMAX && zmax == -INFINITY);  // nothing to divide by
+  // the error of a near score in units of 2^-24 of the largest one: 20 of its own steps, 2 |z| of the exponential's argument (4 |z|
+  // for softmax's difference, whose sum adds one per expert of a lane and a few), 6 |z| where a temperature rounds z; a key's own
+  // rounding comes on top where it is used
+  float delta = 0.f;
+  if (a.bias || a.two) {
+    const float largest = SCORE == DST_SCORE_SOFTMAX ? inv_sum : SCORE == DST_SCORE_SIGMOID ? 1.f : sqrtf(fmaxf(zmax * inv_temp, 0.f) + 0.7f);
+    const float per_z = (SCORE == DST_SCORE_SOFTMAX ? 4.f : 2.f) + (inv_temp == 1.f ? 0.f : 6.f);
+    const float low = value_of(~seg_max(~order_of(zmin)));  // the smallest finite one; an infinity where there is none
+    const float far = fmaxf(fabsf(zmax) < INFINITY ? fabsf(zmax) : 0.f, low < INFINITY ? fabsf(low) : 0.f) * inv_temp;
+    delta = largest * (20.f + (SCORE == DST_SCORE_SOFTMAX ? a.chunk + 8.f : 0.f) + per_z * far) * 0x1p-24f;
+  }
+
+  // groups
+  if (a.kept < a.groups) {
+    uint32_t m1 = top[0], m2 = top[1];
+    for (int off = 1; off < (1 << a.shift); off <<= 1) {
+      const uint32_t o1 = __shfl_xor_sync(FULL, m1, off), o2 = __shfl_xor_sync(FULL, m2, off);
+      m2 = max(min(m1, o1), max(m2, o2));
+      m1 = max(m1, o1);
+    }
+    uint32_t g = m1;
+    const bool sums = a.two && a.size > 1, in = group < a.groups;
+    if (sums && in) g = order_of(a.bias ? value_of(m1) + value_of(m2) : near(value_of(m1)) + near(value_of(m2)));
+    int better = 0;
+    for (int h = 0; h < a.groups; ++h) {
+      const uint32_t o = __shfl_sync(FULL, g, h << a.shift, LPT);
+      better += o > g || (o == g && h < group);
+    }
+    const bool keep = in && better < a.kept;
+    if (sums || a.bias) {  // how near the border is
+      const uint32_t last = ~seg_max(keep ? ~g : 0u), next = seg_max(in && !keep ? g : 0u);
+      const float l = value_of(last), x = value_of(next), tol = (sums ? 4.f : 2.f) * delta + 0x1p-22f * fabsf(l);
+      const bool border = !(l - x > tol);
+      if (__any_sync(FULL, border)) {
+        // groups this near that hold the same two logits are equal indeed
+        const bool close = border && in && fabsf(value_of(g) - l) <= tol;
+        const int ref = __ffs(__ballot_sync(FULL, close) & segment) - 1;
+        const uint32_t r1 = __shfl_sync(FULL, m1, max(ref, 0)), r2 = __shfl_sync(FULL, m2, max(ref, 0));
+        const bool other = seg_any(close && (m1 != r1 || m2 != r2));
+        again = again || (border && (a.bias || ref < 0 || other));
+      }
+    }
+    if (!keep) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top[i] = 0;
+    }
+  }
+
+  uint32_t number = 0, before = 0;  // of pick `tl`; of the round before
+  int from = 0, win_before = -1, run = 0, nth = 0;  // the lane that had it, as its run-th of that number
+  for (int r = 0; r < a.top_k; ++r) {
+    const uint32_t best = seg_max(top[0]);
+    const int win = __ffs(__ballot_sync(FULL, top[0] == best) & segment) - 1;
+    run = best == before && win == win_before ? run + 1 : 0;
+    before = best, win_before = win;
+    if (tl == r) number = best, from = win, nth = run;
     if (lane == win) {
 #pragma unroll
-      for (int j = 0; j < PL; ++j)
-        if (j == at) rank[j] = 0;
+      for (int i = 0; i < 7; ++i) top[i] = top[i + 1];
+      top[7] = 0;
     }
-    w = __shfl_sync(0xffffffffu, w, win);
-    const int id = __shfl_sync(0xffffffffu, id0 + at, win);
-    if (lane == r) my_w = w, my_id = id;
-    wsum += w;
   }
-  if (lane < a.top_k) {
-    a.weights[t * a.top_k + lane] = (float)((a.renorm && a.top_k > 1 ? my_w / (wsum + 1e-20) : my_w) * (double)a.scale);
-    a.ids[t * a.top_k + lane] = my_id;
+  const bool pick = tl < a.top_k;
+  from &= LPT - 1;
+  int at = 0;
+  __syncwarp();
+  const uint32_t* theirs = mine + from * a.stride_s;
+  for (int j0 = ((a.chunk - 1) & ~3); j0 >= 0; j0 -= 4) {  // from behind: the match that is left at the end is the first
+    const uint4 v = *reinterpret_cast<const uint4*>(theirs + j0);
+    at = v.w == number ? j0 + 3 : at;
+    at = v.z == number ? j0 + 2 : at;
+    at = v.y == number ? j0 + 1 : at;
+    at = v.x == number ? j0 : at;
   }
+  for (; nth > 0; --nth) {
+    ++at;
+    while (at < a.chunk - 1 && theirs[at] != number) ++at;
+  }
+  const int id = min((from >> a.shift) * a.size + (from & ((1 << a.shift) - 1)) * a.chunk + at, a.E - 1);
+  float zi = pick ? load_logit(a, row + id) : 0.f;
+  if (flip) zi = -zi;
+
+  if (a.bias) {
+    // picks in the right order: each further above the next than both errors, or of the same logit and bias
+    const float key = value_of(number), b = pick ? a.bias[id] : 0.f;
+    const float tol = 2.f * delta + 0x1p-22f * fabsf(key);
+    const float next_key = __shfl_down_sync(FULL, key, 1, LPT), next_z = __shfl_down_sync(FULL, zi, 1, LPT), next_b = __shfl_down_sync(FULL, b, 1, LPT);
+    const bool unsure = tl + 1 < a.top_k && !(key - next_key > tol) && !(zi == next_z && b == next_b);
+    // and the last one above what is left; a lane whose list ran out may have had more
+    const float last = __shfl_sync(FULL, key, a.top_k - 1, LPT), last_tol = __shfl_sync(FULL, tol, a.top_k - 1, LPT);
+    const uint32_t left = seg_max(top[0]);
+    const int first_from = __shfl_sync(FULL, from, 0, LPT);
+    const bool one_lane = !seg_any(pick && from != first_from);
+    const bool any_unsure = seg_any(unsure);
+    again = again || any_unsure || (a.top_k == 8 && a.chunk > 8 && one_lane);
+    const bool border = left && !(last - value_of(left) > last_tol);
+    if (__any_sync(FULL, border && !again)) {  // equal logits and biases at the border are no matter
+      const float last_z = __shfl_sync(FULL, zi, a.top_k - 1, LPT), last_b = __shfl_sync(FULL, b, a.top_k - 1, LPT);
+      bool other = false;
+      if (border && top[0])
+        for (int j = 0; j < n; ++j) {
+          const float k = value_of(own[j]);
+          if (!(last - k > last_tol) && !(k - last > last_tol)) {
+            const float zj = load_logit(a, row + id0 + j);
+            other = other || (flip ? -zj : zj) != last_z || a.bias[id0 + j] != last_b;
+          }
+        }
+      const bool any_other = seg_any(other);
+      again = again || any_other;
+    }
+  }
+  const float zt = inv_temp == 1.f ? zi : zi / fabsf(a.temp);
+  float w = 0.f;
+  if (pick) {
+    if (SCORE == DST_SCORE_SOFTMAX) w = expf(zt - (inv_temp == 1.f ? zmax : zmax / fabsf(a.temp))) * inv_sum;
+    else w = score_of<SCORE>(zt);
+  }
+  if (a.renorm && a.top_k > 1) {
+    float wsum = w;
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) wsum += __shfl_xor_sync(FULL, wsum, off);
+    w = w / (wsum + 1e-20f);
+  }
+  if (pick && valid && !again) {
+    a.weights[t * a.top_k + tl] = w * a.scale;
+    a.ids[t * a.top_k + tl] = id;
+  }
+  return again && valid;
 }
 
-template <int PL, typename T>
-__global__ void __launch_bounds__(128) route_group_kernel(const GroupRoute a) {
-  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (t < a.T) route_token<PL, T>(a, t, threadIdx.x & 31);
+template <int SCORE, int LPT>
+__global__ void __launch_bounds__(WARPS * 32) route_group_kernel(const GroupRoute a) {
+  extern __shared__ uint4 shared[];  // the tokens' numbers, then over them the keys of one in 64 bits
+  constexpr int TOKENS = WARPS * 32 / LPT;
+  __shared__ double red[WARPS];
+  __shared__ int again[TOKENS];
+  const int at = threadIdx.x / LPT;
+  const int64_t t0 = (int64_t)blockIdx.x * TOKENS, t = t0 + at;
+  const bool valid = t < a.T;
+  const bool exact = route_tokens<SCORE, LPT>(a, valid ? t : a.T - 1, valid, reinterpret_cast<uint32_t*>(shared) + at * LPT * a.stride_s);
+  if (threadIdx.x % LPT == 0) again[at] = exact;
+  if (!__syncthreads_or(exact)) return;
+  for (int i = 0; i < TOKENS; ++i)
+    if (again[i]) route_exact<SCORE>(a, t0 + i, reinterpret_cast<uint64_t*>(shared), red);
 }
 
-template <typename T>
-int launch(const GroupRoute& a, cudaStream_t st) {
-  const unsigned grid = (unsigned)cdiv64(a.T, 4);
-  if (a.chunk <= 4) route_group_kernel<4, T><<<grid, 128, 0, st>>>(a);
-  else if (a.chunk <= 8) route_group_kernel<8, T><<<grid, 128, 0, st>>>(a);
-  else if (a.chunk <= 16) route_group_kernel<16, T><<<grid, 128, 0, st>>>(a);
-  else route_group_kernel<64, T><<<grid, 128, 0, st>>>(a);
+template <int SCORE, int LPT>
+int launch(GroupRoute a, cudaStream_t st) {
+  int wide = 0;
+  while ((1 << wide) < a.groups) ++wide;
+  a.shift = 0;
+  while ((1 << (a.shift + wide)) < LPT) ++a.shift;
+  a.chunk = (a.size + (1 << a.shift) - 1) >> a.shift;
+  const int pieces = (a.chunk + 3) / 4 + (a.chunk % 8 != 0 && a.chunk % 8 <= 4);  // whole eights can be read
+  a.stride_s = 4 * (pieces | 1);
+  a.vec = a.dtype == DST_OUT_F32 && a.chunk % 4 == 0 && a.chunk >= 8 && a.size == a.chunk << a.shift && a.stride % 4 == 0 &&
+          reinterpret_cast<uintptr_t>(a.logits) % 16 == 0;
+  a.vec_bias = a.chunk % 8 == 0 && a.size == a.chunk << a.shift && reinterpret_cast<uintptr_t>(a.bias) % 16 == 0;
+  a.per_lane = a.vec ? (uint32_t)(((1ull << 32) + a.chunk / 4 - 1) / (a.chunk / 4)) : 0;
+  constexpr int TOKENS = WARPS * 32 / LPT;
+  const size_t numbers = (size_t)TOKENS * LPT * a.stride_s * 4, keys = (size_t)a.E * 8;
+  const size_t smem = numbers > keys ? numbers : keys;  // at most 36 KB (sixteen lanes with 64 experts each)
+  route_group_kernel<SCORE, LPT><<<(unsigned)cdiv64(a.T, TOKENS), WARPS * 32, smem, st>>>(a);
   DST_CUDA_TRY(cudaGetLastError());
   return DST_OK;
+}
+
+template <int SCORE>
+int launch_for(const GroupRoute& a, cudaStream_t st) {
+  // A warp for each token as long as all of them run at once; then several tokens a warp, which share the steps across lanes.
+  // 384 experts in eight groups, top-6 (8) with sums and a bias, us for 777 / 16 384 tokens: a warp each 5.6 / 40.7 (44), two a warp
+  // 7.1 / 32.9 (36), four a warp 10.4 / 33.5 (35); without a bias and by the largest (top-8) two 18, four 14
+  if (a.groups > 16 || a.T <= 32 * (int64_t)sm_count()) return launch<SCORE, 32>(a, st);
+  if (a.groups > 8 || a.E > 512) return launch<SCORE, 16>(a, st);
+  return launch<SCORE, 8>(a, st);
 }
 
 }  // namespace
@@ -165,17 +510,14 @@ extern "C" int dst_route_group_topk(const void* logits, int logits_dtype, int64_
     return DST_ERR_BAD_ARG;
   if (E % n_groups != 0 || topk_groups > n_groups || row_stride < E || T > 0x7fffffff) return DST_ERR_BAD_SHAPE;
   const int size = (int)(E / n_groups);
-  if (E > 1024 || n_groups > 32 || top_k > 8 || (int64_t)top_k > (int64_t)topk_groups * size) return DST_ERR_UNSUPPORTED;
+  if (E > 1024 || n_groups > 32 || top_k > TOP || (int64_t)top_k > (int64_t)topk_groups * size) return DST_ERR_UNSUPPORTED;
   if (T == 0) return DST_OK;
   if (!logits || !weights || !ids) return DST_ERR_BAD_ARG;
   GroupRoute a{};
   a.logits = logits, a.stride = row_stride, a.bias = bias, a.T = T, a.E = (int)E, a.groups = n_groups, a.size = size;
-  a.lanes = 32;
-  while (a.lanes * n_groups > 32) a.lanes >>= 1;
-  a.chunk = (size + a.lanes - 1) / a.lanes;  // at most 60: 17 groups of 60 on a lane each
-  a.kept = topk_groups, a.two = group_score == DST_GROUP_TOP2, a.top_k = top_k, a.score = score_func, a.renorm = renorm;
+  a.kept = topk_groups, a.two = group_score == DST_GROUP_TOP2, a.top_k = top_k, a.renorm = renorm, a.dtype = logits_dtype;
   a.temp = gate_temp, a.scale = route_scale, a.weights = weights, a.ids = ids;
   auto st = static_cast<cudaStream_t>(stream);
-  if (logits_dtype == DST_OUT_F32) return launch<float>(a, st);
-  return logits_dtype == DST_OUT_BF16 ? launch<__nv_bfloat16>(a, st) : launch<__half>(a, st);
+  if (score_func == DST_SCORE_SOFTMAX) return launch_for<DST_SCORE_SOFTMAX>(a, st);
+  return score_func == DST_SCORE_SIGMOID ? launch_for<DST_SCORE_SIGMOID>(a, st) : launch_for<DST_SCORE_SQRTSOFTPLUS>(a, st);
 }
