@@ -20,7 +20,7 @@ from ..kernels import ternary_b200 as kb
 
 _UNAVAILABLE = "the B200 adapters are unavailable: {} not on a CUDA device and this backend has no CPU path"
 _PADDED_RANKS = (16, 32, 64, 128)
-_TILE = 16
+_EXPERT_TILE = 16
 
 
 def _int32(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -62,10 +62,11 @@ class AdapterPlan:
                 raise RuntimeError("offsets and slots must share one device")
         if n_adapters < 1 or n_adapters > 4095 or n_rows < 0:
             raise RuntimeError("a plan takes 1 to 4095 adapters")
-        self.n_rows, self.n_adapters, self.tile, self.device = n_rows, n_adapters, _TILE, dev
-        self.max_tiles = min(n_rows, -(-n_rows // _TILE) + n_adapters + 1)
+        self.n_rows, self.n_adapters, self.device = n_rows, n_adapters, dev
+        tile = self.tile = int(lib.dst_adapter_tile(n_rows))
+        self.max_tiles = min(n_rows, -(-n_rows // tile) + n_adapters + 1)
         # one buffer: tiles, order, bins, offsets
-        at_order = int(lib.dst_adapter_tile_capacity(n_rows, n_adapters + 1, _TILE))
+        at_order = int(lib.dst_adapter_tile_capacity(n_rows, n_adapters + 1, tile))
         at_bins, at_offsets = at_order + n_rows, at_order + 2 * n_rows
         self._buf = torch.empty(at_offsets + n_adapters + 2, dtype=torch.int32, device=dev)
         self._at = at_order, at_bins, at_offsets
@@ -74,9 +75,9 @@ class AdapterPlan:
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         with kb._guard(dev):
             _lib.check(lib.dst_adapter_plan(offsets.data_ptr() if offsets is not None else None, slots.data_ptr(), slots.size(0), n_rows, n_adapters,
-                                            _TILE, base + 4 * at_order, base + 4 * at_bins, base + 4 * at_offsets, base,
+                                            tile, base + 4 * at_order, base + 4 * at_bins, base + 4 * at_offsets, base,
                                             ws.data_ptr() if ws is not None else None, ws_bytes, kb._stream(slots)))
-        self._c = _lib.AdapterRowsC(rows=base + 4 * at_order, x_rows=base + 4 * at_order, tiles=base, max_tiles=self.max_tiles, tile=_TILE)
+        self._c = _lib.AdapterRowsC(rows=base + 4 * at_order, x_rows=base + 4 * at_order, tiles=base, max_tiles=self.max_tiles, tile=tile)
         self._ref = ctypes.byref(self._c)
 
     @property
@@ -106,21 +107,21 @@ class ExpertPlan:
         ids = _int32(ids, "expert ids")
         T, k = ids.shape
         P, n, dev = T * k, plan.n_adapters, plan.device
-        self.tokens, self.n_rows, self.n_adapters, self.n_experts, self.tile, self.device = T, P, n, n_experts, _TILE, dev
-        self.max_tiles = min(P, -(-P // _TILE) + (n + 1) * n_experts)
+        self.tokens, self.n_rows, self.n_adapters, self.n_experts, self.tile, self.device = T, P, n, n_experts, _EXPERT_TILE, dev
+        self.max_tiles = min(P, -(-P // _EXPERT_TILE) + (n + 1) * n_experts)
         self.order = torch.empty(P, dtype=torch.int64, device=dev)
         self.offsets = torch.empty(n_experts + 1, dtype=torch.int64, device=dev)
-        cap = int(lib.dst_adapter_tile_capacity(P, (n + 1) * n_experts, _TILE))
+        cap = int(lib.dst_adapter_tile_capacity(P, (n + 1) * n_experts, _EXPERT_TILE))
         self._buf = torch.empty(cap + P, dtype=torch.int32, device=dev)
         ws_bytes = int(lib.dst_adapter_plan_experts_workspace_bytes(P, n_experts))
         ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
         base, src = self._buf.data_ptr(), plan._buf.data_ptr()
         with kb._guard(dev):
-            _lib.check(lib.dst_adapter_plan_experts(ids.data_ptr(), T, k, n_experts, src + 4 * plan._at[0], src + 4 * plan._at[1], n, _TILE,
+            _lib.check(lib.dst_adapter_plan_experts(ids.data_ptr(), T, k, n_experts, src + 4 * plan._at[0], src + 4 * plan._at[1], n, _EXPERT_TILE,
                                                     self.order.data_ptr(), self.offsets.data_ptr(), base + 4 * cap, base, ws.data_ptr(), ws_bytes,
                                                     kb._stream(ids)))
-        self._pairs = _lib.AdapterRowsC(rows=None, x_rows=None, tiles=base, max_tiles=self.max_tiles, tile=_TILE)
-        self._tokens = _lib.AdapterRowsC(rows=None, x_rows=base + 4 * cap, tiles=base, max_tiles=self.max_tiles, tile=_TILE)
+        self._pairs = _lib.AdapterRowsC(rows=None, x_rows=None, tiles=base, max_tiles=self.max_tiles, tile=_EXPERT_TILE)
+        self._tokens = _lib.AdapterRowsC(rows=None, x_rows=base + 4 * cap, tiles=base, max_tiles=self.max_tiles, tile=_EXPERT_TILE)
 
 
 class LowRankAdapters:
@@ -144,8 +145,10 @@ class LowRankAdapters:
             raise RuntimeError(_UNAVAILABLE.format("the adapters are"))
         self.n_adapters, self.K, self.N, self.rank, self.dtype, self.experts, self.parts = n_adapters, K, N, rank, dtype, experts, parts
         E, Kp = experts or 1, -(-K // 32) * 32
-        self._a = torch.zeros(n_adapters, E, parts, self.rank_padded, Kp, dtype=dtype, device=device)
-        self._b = torch.zeros(n_adapters, E, N, self.rank_padded, dtype=dtype, device=device)
+        # A in steps of 32 values of K, the ranks of a step together: what a warp reads at once is one stretch of memory
+        self._a = torch.zeros(n_adapters, E, Kp // 32, parts, self.rank_padded, 32, dtype=dtype, device=device)
+        rows = n_adapters * E * N  # and 31 more, which the last step of columns may read
+        self._b = torch.zeros(rows + 31, self.rank_padded, dtype=dtype, device=device)[:rows].view(n_adapters, E, N, self.rank_padded)
         self._scale = torch.zeros(n_adapters, dtype=torch.float32, device=device)
         self._ranks = torch.zeros(n_adapters, dtype=torch.int32, device=device)
         self.device = self._a.device
@@ -162,7 +165,9 @@ class LowRankAdapters:
         if tuple(A.shape) != (*lead, self.parts * r, self.K) or tuple(B.shape) != (*lead, self.N, r) or not 1 <= r <= self.rank:
             raise RuntimeError("inconsistent adapter shapes")
         self.clear(slot)
-        self._a[slot, ..., :r, :self.K] = A.reshape(-1, self.parts, r, self.K)
+        wide = torch.zeros(A.numel() // (self.parts * r * self.K), self.parts, r, self._a.size(2) * 32, dtype=self.dtype, device=self.device)
+        wide[..., :self.K] = A.reshape(-1, self.parts, r, self.K)
+        self._a[slot, ..., :r, :] = wide.unflatten(-1, (-1, 32)).permute(0, 3, 1, 2, 4)
         self._b[slot, ..., :r] = B.reshape(-1, self.N, r)
         self._scale[slot] = scale
         self._ranks[slot] = r

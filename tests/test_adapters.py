@@ -95,6 +95,21 @@ def test_route_groups_types_strides_and_options(T, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("E,groups,kept,k,score,group_score,with_bias", [(384, 8, 4, 6, "sqrtsoftplus", "top2", True), (256, 8, 4, 8, "sigmoid", "top2", False),
+                                                                         (96, 6, 2, 8, "softmax", "top2", True), (160, 16, 5, 4, "softmax", "max", False),
+                                                                         (640, 4, 2, 8, "sigmoid", "max", True), (63, 7, 7, 8, "sigmoid", "max", True)])
+def test_route_groups_many_tokens(E, groups, kept, k, score, group_score, with_bias):
+    """Several tokens share a warp; among them some with masked experts, NaNs and equal logits."""
+    g = gen(E)
+    logits = torch.randn(6000, E, generator=g, device=DEV)
+    logits[::7] = logits[::7].to(BF16).float()
+    logits[5::50, ::3] = -torch.inf
+    logits[9::500, 1] = torch.nan
+    bias = torch.randn(E, generator=g, device=DEV) * 0.05 if with_bias else None
+    check_route(logits, k, 1.0, True, score, bias, 1.0, groups, kept, group_score)
+
+
+@gpu
 def test_route_groups_ties_go_to_the_lower_index():
     g = gen(5)
     check_route(torch.randint(-2, 3, (200, 128), generator=g, device=DEV).float(), 8, groups=8, kept=3)
