@@ -1,10 +1,17 @@
-// Plans for the low-rank adapters: rows sorted by the adapter of their request, cut into tiles of rows of one adapter.
+// Plans for the low-rank adapters: rows sorted by the adapter of their request, cut into tiles of rows of one adapter; the pairs
+// (token, choice) of a MoE layer sorted by expert and adapter.
 //
 // A bin is an adapter 0 .. n-1, or n for the rows without one (request without an adapter, an adapter outside [0, n), a row
-// behind the last request). The rows of a bin keep their order (a stable counting sort), so a plan depends on its input alone.
+// behind the last request). The rows of a bin keep their order (a stable sort), so a plan depends on its input alone.
 //
 // Tile list, int32: [0] count, [1..3] unused, then count + 1 pairs (first position, matrix); a tile ends where the next one
 // starts, matrix -1: rows without an adapter.
+//
+// A few microseconds of latency are all there is to win here: up to 1024 entries are ranked by one block, more by one cluster of
+// up to eight blocks (a counting sort whose blocks exchange their counts through the cluster's shared memory), and only what
+// does not fit there goes through the routing sort's kernels.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "dst_common.cuh"
@@ -12,7 +19,13 @@
 namespace dst {
 namespace {
 
-constexpr int PLAN_THREADS = 1024, PLAN_WARPS = 32, PLAN_ROWS = 16384, PLAN_BINS = 1024;  // of the one-block forms
+namespace cg = cooperative_groups;
+
+constexpr int THREADS = 1024, WARPS = 32, SMALL = 1024, MAX_CTAS = 8;
+constexpr int64_t CLUSTER_ENTRIES = 131072;  // entries and bins of the cluster's form
+constexpr int CLUSTER_BINS = 1024;
+constexpr int64_t RANK_ROWS = 192, RANK_PAIRS = 384;  // beyond, a cluster is faster: 128 / 256 / 1024 rows 4.6 / 5.9 / 27 us against 5.8 / 5.8 / 6.3,
+                                                        // 256 / 512 pairs (with their adapters) 10.0 / 14.3 against 13.1 / 14.3
 
 // The bin of a row: the request that it lies in is the last one that starts at or before it.
 __device__ __forceinline__ int bin_of_row(const int32_t* __restrict__ offsets, const int32_t* __restrict__ slots, int64_t requests, int64_t row,
@@ -32,111 +45,292 @@ __device__ __forceinline__ int bin_of_row(const int32_t* __restrict__ offsets, c
   return s >= 0 && s < n ? s : n;
 }
 
-// Exclusive sums of val[0 .. count) in place by the whole block, count <= 1024 per pass of its threads; returns the total.
+// Exclusive sum of v over the threads of the block; `total`: of all
 __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (int)(blockDim.x >> 5);
   int incl = v;
+#pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const int up = __shfl_up_sync(0xffffffffu, incl, d);
     if (lane >= d) incl += up;
   }
   if (lane == 31) warp_sums[warp] = incl;
   __syncthreads();
-  int before = 0;
-  total = 0;
-  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
-    if (w < warp) before += warp_sums[w];
-    total += warp_sums[w];
+  int w = lane < warps ? warp_sums[lane] : 0;
+  const int own = w;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, w, d);
+    if (lane >= d) w += up;
   }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w - own, warp);
   __syncthreads();
   return before + incl - v;
 }
 
-// The whole plan by one block: each warp counts and places a run of consecutive rows of its own.
-__global__ void __launch_bounds__(PLAN_THREADS)
-plan_kernel(const int32_t* __restrict__ offsets, const int32_t* __restrict__ slots, int64_t requests, int rows, int n, int tile,
-            int32_t* __restrict__ order, int32_t* __restrict__ bins, int32_t* __restrict__ bin_offsets, int32_t* __restrict__ tiles) {
-  extern __shared__ int32_t sh[];
-  const int nb = n + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int32_t* hist = sh;                       // [PLAN_WARPS][nb]
-  int32_t* start = hist + PLAN_WARPS * nb;  // [nb + 1]
-  int32_t* tstart = start + nb + 1;         // [nb + 1]
-  uint16_t* bin_s = reinterpret_cast<uint16_t*>(tstart + nb + 1);  // [rows]
-  __shared__ int sums[32];
-  for (int i = tid; i < PLAN_WARPS * nb; i += PLAN_THREADS) hist[i] = 0;
-  __syncthreads();
-  const int per = ((rows + PLAN_WARPS - 1) / PLAN_WARPS + 31) & ~31;
-  const int r0 = min(warp * per, rows), r1 = min(r0 + per, rows);
-  int32_t* mine = hist + warp * nb;
-  for (int r = r0; r < r1; r += 32) {
-    const bool in = r + lane < r1;
-    const int b = in ? bin_of_row(offsets, slots, requests, r + lane, n) : -1;
-    const unsigned peers = __match_any_sync(0xffffffffu, b);
-    if (in) {
-      bin_s[r + lane] = (uint16_t)b;
-      if (lane == __ffs(peers) - 1) mine[b] += __popc(peers);
+// What is sorted: the rows of a batch by bin (ids null), or the pairs of a MoE layer by expert and bin
+struct Plan {
+  const int32_t *offsets, *slots;  // rows: requests (offsets null: a slot per row)
+  int64_t requests;
+  const int32_t *ids, *row_order, *row_bins;  // pairs: experts [T, k], the tokens' plan
+  int entries, n, k, E, tile;
+  int32_t *order, *bins, *bin_offsets;  // rows
+  int64_t *pair_order, *expert_offsets;  // pairs
+  int32_t *x_rows, *tiles;
+  int32_t* keys;  // pairs by a cluster: expert and bin of each position
+};
+
+// ------------------------------------------------------------------------------------ up to 1024 entries
+// Thread i has entry i: its place is the number of smaller keys and of equal ones before it.
+__global__ void __launch_bounds__(THREADS) small_kernel(const Plan a) {
+  __shared__ __align__(16) int key_s[SMALL];
+  __shared__ int sorted[SMALL], sums[32];
+  const int i = threadIdx.x, n1 = a.n + 1;
+  constexpr int DROPPED = 0x7fffffff;
+  int key = DROPPED, b = a.n;
+  if (i < a.entries) {
+    if (a.ids) {
+      const int e = a.ids[i];
+      b = a.row_bins[i / a.k];
+      if (e >= 0 && e < a.E) key = e * n1 + b;
+    } else {
+      key = b = bin_of_row(a.offsets, a.slots, a.requests, i, a.n);
+      a.bins[i] = b;
     }
-    __syncwarp();
+  }
+  key_s[i] = key;
+  __syncthreads();
+  int place = 0;
+  const int quads = (a.entries + 3) / 4, own = i / 4;  // entries behind the last are DROPPED and come last
+  const int4* four = reinterpret_cast<const int4*>(key_s);
+#pragma unroll 4
+  for (int q = 0; q < quads; ++q) {  // up to an equal one before it; equal ones behind it do not count
+    const int4 v = four[q];
+    const int limit = q < own ? key : key - 1;
+    place += (v.x <= limit) + (v.y <= limit) + (v.z <= limit) + (v.w <= limit);
+  }
+  for (int j = own * 4; j < i; ++j) place += key_s[j] == key;  // those of its own four
+  if (i < a.entries) {
+    sorted[place] = key;
+    if (a.ids) {
+      a.pair_order[place] = key == DROPPED ? -1 : i;
+      a.x_rows[place] = key == DROPPED ? 0 : i / a.k;
+    } else {
+      a.order[place] = i;
+    }
   }
   __syncthreads();
-  int count = 0;
-  if (tid < nb)
-    for (int w = 0; w < PLAN_WARPS; ++w) {
-      const int v = hist[w * nb + tid];
-      hist[w * nb + tid] = count;
-      count += v;
-    }
-  int total, n_tiles;
-  const int at = block_scan(count, sums, total);
-  const int tat = block_scan((count + tile - 1) / tile, sums, n_tiles);
-  if (tid < nb) start[tid] = at, tstart[tid] = tat, bin_offsets[tid] = at;
-  if (tid == 0) start[nb] = rows, tstart[nb] = n_tiles, bin_offsets[nb] = rows, tiles[0] = n_tiles;
-  __syncthreads();
-  int2* list = reinterpret_cast<int2*>(tiles + 4);
-  for (int i = tid; i <= n_tiles; i += PLAN_THREADS) {
-    int lo = 0, hi = nb;  // the last bin whose tiles start at or before i and which has some
+  const auto first_at_least = [&](int k) {
+    int lo = 0, hi = a.entries;
     while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (mid <= nb - 1 && tstart[mid] <= i) lo = mid;
-      else hi = mid - 1;
+      const int mid = (lo + hi) >> 1;
+      if (sorted[mid] < k) lo = mid + 1;
+      else hi = mid;
     }
-    list[i] = i == n_tiles ? make_int2(rows, -1) : make_int2(start[lo] + (i - tstart[lo]) * tile, lo < n ? lo : -1);
+    return lo;
+  };
+  if (a.ids) {
+    for (int e = i; e <= a.E; e += blockDim.x) a.expert_offsets[e] = first_at_least(e * n1);
+  } else {
+    for (int v = i; v <= n1; v += blockDim.x) a.bin_offsets[v] = first_at_least(v);
   }
-  for (int r = r0; r < r1; r += 32) {
-    const bool in = r + lane < r1;
-    const int b = in ? (int)bin_s[r + lane] : -1;
-    const unsigned peers = __match_any_sync(0xffffffffu, b);
-    if (in) {
-      const int p = start[b] + mine[b] + __popc(peers & ((1u << lane) - 1u));
-      order[p] = r + lane;
-      bins[p] = b;
-    }
-    __syncwarp();
-    if (in && lane == __ffs(peers) - 1) mine[b] += __popc(peers);
-    __syncwarp();
+  const int mine = i < a.entries ? sorted[i] : DROPPED;
+  const bool starts = mine != DROPPED && (i - first_at_least(mine)) % a.tile == 0;
+  int total;
+  const int at = block_scan(starts, sums, total);
+  const int valid = __syncthreads_count(mine != DROPPED);
+  int2* list = reinterpret_cast<int2*>(a.tiles + 4);
+  if (starts) {
+    const int e = mine / n1, bin = mine - e * n1;  // rows: the key is the bin
+    list[at] = make_int2(i, bin == a.n ? -1 : bin * (a.ids ? a.E : 1) + (a.ids ? e : 0));
+  }
+  if (i == 0) {
+    a.tiles[0] = total;
+    list[total] = make_int2(valid, -1);
   }
 }
 
-// More rows or adapters: the bins, the routing sort over them, then the lists from its result.
+// ------------------------------------------------------------------------------------ one cluster
+// A warp counts and places a run of consecutive entries of its own. Rows: keys are bins. Pairs: taken in the order of the tokens'
+// plan, which is the bins', and sorted by expert; a tile starts where expert or bin change and at multiples of its height.
+template <bool PAIRS>
+__global__ void __launch_bounds__(THREADS) cluster_kernel(const Plan a) {
+  extern __shared__ int32_t sh[];
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
+  const int nb = PAIRS ? a.E : a.n + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int32_t* totals = sh;                   // [nb] this block's, read by the others
+  int32_t* start = totals + nb;           // [nb] of this block's entries
+  int32_t* global = start + nb;           // [nb + 1] of all
+  int32_t* tstart = global + nb + 1;      // [nb + 1] rows: first tile of a bin
+  uint16_t* hist = reinterpret_cast<uint16_t*>(tstart + nb + 1);  // [WARPS][nb]
+  uint16_t* key_s = hist + WARPS * nb;                            // [entries of the block]
+  __shared__ int sums[32], tile_total;
+  const int run = ((a.entries + ctas * WARPS - 1) / (ctas * WARPS) + 31) & ~31;
+  const int e0 = min((cta * WARPS + warp) * run, a.entries), e1 = min(e0 + run, a.entries), block0 = cta * WARPS * run;
+  for (int i = tid; i < WARPS * nb / 2 + 1; i += THREADS) reinterpret_cast<uint32_t*>(hist)[i] = 0;
+  __syncthreads();
+  uint16_t* mine = hist + warp * nb;
+  constexpr int NONE = 0xffff;
+  for (int q = e0; q < e1; q += 32) {
+    const int i = q + lane;
+    int key = NONE;
+    if (i < e1) {
+      if (PAIRS) {
+        const int e = a.ids[(int64_t)a.row_order[i / a.k] * a.k + i % a.k];
+        key = e >= 0 && e < a.E ? e : NONE;
+      } else {
+        key = bin_of_row(a.offsets, a.slots, a.requests, i, a.n);
+        a.bins[i] = key;
+      }
+      key_s[i - block0] = (uint16_t)key;
+    }
+    const unsigned peers = __match_any_sync(0xffffffffu, key);
+    if (key != NONE && lane == __ffs(peers) - 1) mine[key] += (uint16_t)__popc(peers);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int b = tid; b < nb; b += THREADS) {  // each warp's first place among the block's
+    int count = 0;
+#pragma unroll 8
+    for (int w = 0; w < WARPS; ++w) {
+      const int v = hist[w * nb + b];
+      hist[w * nb + b] = (uint16_t)count;
+      count += v;
+    }
+    totals[b] = count;
+  }
+  cluster.sync();
+  int all = 0, before = 0;
+  if (tid < nb) {
+#pragma unroll
+    for (int c = 0; c < MAX_CTAS; ++c) {
+      const int v = c < ctas ? cluster.map_shared_rank(totals, c)[tid] : 0;
+      all += v;
+      before += c < cta ? v : 0;
+    }
+  }
+  int valid, n_tiles = 0;
+  const int at = block_scan(all, sums, valid);
+  if (tid < nb) start[tid] = at + before, global[tid] = at;
+  if (tid == 0) global[nb] = valid;
+  if (PAIRS) {
+    if (cta == 0)
+      for (int b = tid; b <= nb; b += THREADS) a.expert_offsets[b] = b < nb ? (tid < nb ? at : 0) : valid;
+  } else {
+    const int tat = block_scan((all + a.tile - 1) / a.tile, sums, n_tiles);
+    if (tid < nb) tstart[tid] = tat;
+    if (tid == 0) tstart[nb] = n_tiles;
+    if (cta == 0) {
+      if (tid < nb) a.bin_offsets[tid] = at;
+      if (tid == 0) a.bin_offsets[nb] = a.entries, a.tiles[0] = n_tiles;
+    }
+  }
+  __syncthreads();
+  int2* list = reinterpret_cast<int2*>(a.tiles + 4);
+  if (!PAIRS) {
+    for (int i = cta * THREADS + tid; i <= n_tiles; i += ctas * THREADS) {
+      int lo = 0, hi = nb - 1;  // the last bin whose tiles start at or before i
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tstart[mid] <= i) lo = mid;
+        else hi = mid - 1;
+      }
+      list[i] = i == n_tiles ? make_int2(a.entries, -1) : make_int2(global[lo] + (i - tstart[lo]) * a.tile, lo < a.n ? lo : -1);
+    }
+  }
+  for (int q = e0; q < e1; q += 32) {
+    const int i = q + lane, key = i < e1 ? (int)key_s[i - block0] : NONE;
+    const unsigned peers = __match_any_sync(0xffffffffu, key);
+    if (key != NONE) {
+      const int p = start[key] + mine[key] + __popc(peers & ((1u << lane) - 1u));
+      if (PAIRS) {
+        const int token = a.row_order[i / a.k];
+        a.pair_order[p] = (int64_t)token * a.k + i % a.k;
+        a.x_rows[p] = token;
+        const int bin = a.row_bins[token];
+        a.keys[p] = bin < a.n ? bin * a.E + key : -1 - key;  // the matrix; without an adapter a negative number per expert
+      } else {
+        a.order[p] = i;
+      }
+    }
+    __syncwarp();
+    if (key != NONE && lane == __ffs(peers) - 1) mine[key] += (uint16_t)__popc(peers);
+    __syncwarp();
+  }
+  if (PAIRS) {
+    for (int p = valid + cta * THREADS + tid; p < a.entries; p += ctas * THREADS) a.pair_order[p] = -1, a.x_rows[p] = 0;
+    cluster.sync();  // the positions' keys of all blocks
+    const int per = (valid + ctas * THREADS - 1) / (ctas * THREADS), p0 = min((cta * THREADS + tid) * per, valid), p1 = min(p0 + per, valid);
+    int starts = 0;
+    for (int p = p0; p < p1; ++p) starts += p % a.tile == 0 || a.keys[p] != a.keys[p - 1];
+    int total;
+    int tat = block_scan(starts, sums, total);
+    if (tid == 0) tile_total = total;
+    cluster.sync();
+    int everything = 0;
+#pragma unroll
+    for (int c = 0; c < MAX_CTAS; ++c) {
+      const int v = c < ctas ? *cluster.map_shared_rank(&tile_total, c) : 0;
+      everything += v;
+      tat += c < cta ? v : 0;
+    }
+    for (int p = p0; p < p1; ++p)
+      if (p % a.tile == 0 || a.keys[p] != a.keys[p - 1]) list[tat++] = make_int2(p, max(a.keys[p], -1));
+    if (cta == 0 && tid == 0) {
+      a.tiles[0] = everything;
+      list[everything] = make_int2(valid, -1);
+    }
+  }
+  cluster.sync();  // nobody leaves while its counts may be read
+}
+
+template <bool PAIRS>
+int launch_cluster(const Plan& a, cudaStream_t st) {
+  const int nb = PAIRS ? a.E : a.n + 1;
+  int ctas = 1;
+  while (ctas < MAX_CTAS && (int64_t)ctas * THREADS < a.entries) ctas *= 2;
+  const int64_t run = (cdiv64(a.entries, ctas * WARPS) + 31) & ~(int64_t)31;
+  const size_t smem = (size_t)(4 * nb + 2) * 4 + (size_t)WARPS * nb * 2 + 4 + (size_t)WARPS * run * 2;
+  constexpr int MOST = (4 * CLUSTER_BINS + 2) * 4 + WARPS * CLUSTER_BINS * 2 + 4 + (int)(CLUSTER_ENTRIES / MAX_CTAS) * 2;  // 113 KB
+  DST_CUDA_TRY(cudaFuncSetAttribute(cluster_kernel<PAIRS>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  DST_CUDA_TRY(cudaLaunchKernelEx(&cfg, cluster_kernel<PAIRS>, a));
+  return DST_OK;
+}
+
+int launch_small(const Plan& a, cudaStream_t st) {
+  const unsigned threads = (unsigned)std::max<int64_t>(128, cdiv64(a.entries, 32) * 32);
+  small_kernel<<<1, threads, 0, st>>>(a);
+  DST_CUDA_TRY(cudaGetLastError());
+  return DST_OK;
+}
+
+// ------------------------------------------------------------------------------------ anything larger
+// The bins, the routing sort over them, then the lists from its result.
 __global__ void bins_kernel(const int32_t* __restrict__ offsets, const int32_t* __restrict__ slots, int64_t requests, int64_t rows, int n,
                             int32_t* __restrict__ bin) {
   const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (r < rows) bin[r] = bin_of_row(offsets, slots, requests, r, n);
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS)
-lists_kernel(const int64_t* __restrict__ order64, const int64_t* __restrict__ offsets64, const int32_t* __restrict__ bin, int64_t rows, int n,
-             int tile, int32_t* __restrict__ order, int32_t* __restrict__ bins, int32_t* __restrict__ bin_offsets, int32_t* __restrict__ tiles) {
+__global__ void __launch_bounds__(THREADS)
+lists_kernel(const int64_t* __restrict__ order64, const int64_t* __restrict__ offsets64, int64_t rows, int n, int tile, int32_t* __restrict__ order,
+             int32_t* __restrict__ bin_offsets, int32_t* __restrict__ tiles) {
   for (int64_t p = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; p < rows; p += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = order64[p];
-    order[p] = (int32_t)r;
-    bins[p] = bin[r];
+    order[p] = (int32_t)order64[p];
   }
   if (blockIdx.x) return;
   __shared__ int sums[32];
   int2* list = reinterpret_cast<int2*>(tiles + 4);
   int done = 0;
-  for (int b0 = 0; b0 <= n; b0 += PLAN_THREADS) {
+  for (int b0 = 0; b0 <= n; b0 += THREADS) {
     const int b = b0 + threadIdx.x;
     const int64_t a = b <= n ? offsets64[b] : 0, e = b <= n ? offsets64[b + 1] : 0;
     int total;
@@ -155,10 +349,7 @@ lists_kernel(const int64_t* __restrict__ order64, const int64_t* __restrict__ of
   }
 }
 
-// ------------------------------------------------------------------------------------ pairs of a MoE layer
-// Pairs (token, choice) sorted by expert and, inside an expert, by bin: the stable routing sort over the pairs in the plan's
-// order of tokens does both, since that order is the bins'. A tile starts where the expert or the bin changes and at every
-// multiple of the tile height.
+// Pairs: the routing sort over them in the order of the tokens' plan, then the tile starts as the cluster finds them
 __global__ void pair_ids_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ order, int64_t pairs, int k, int E,
                                 int32_t* __restrict__ permuted) {
   const int64_t q = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -183,15 +374,15 @@ __device__ __forceinline__ int pair_matrix(const PairLists& a, int64_t p, int64_
   if (q < 0) return -2;
   token = a.order[q / a.k];
   pair = (int64_t)token * a.k + q % a.k;
-  const int b = a.bins[q / a.k], e = a.permuted[q];
+  const int b = a.bins[token], e = a.permuted[q];
   return b < a.n ? b * a.E + e : -1 - 2 * (e + 1);  // no adapter: one negative number per expert
 }
 
 // PLACE false: the tile starts of each block's positions are counted; true: they are written behind those of the blocks before
 template <bool PLACE>
-__global__ void __launch_bounds__(PLAN_THREADS) pair_lists_kernel(const PairLists a) {
+__global__ void __launch_bounds__(THREADS) pair_lists_kernel(const PairLists a) {
   __shared__ int sums[32];
-  const int64_t p = (int64_t)blockIdx.x * PLAN_THREADS + threadIdx.x;
+  const int64_t p = (int64_t)blockIdx.x * THREADS + threadIdx.x;
   bool starts = false;
   int m = -2;
   if (p < a.pairs) {
@@ -209,7 +400,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) pair_lists_kernel(const PairList
     return;
   }
   int before = 0;
-  for (int b = threadIdx.x; b < (int)blockIdx.x; b += PLAN_THREADS) before += a.counts[b];
+  for (int b = threadIdx.x; b < (int)blockIdx.x; b += THREADS) before += a.counts[b];
   int base, unused;
   unused = block_scan(before, sums, base);
   (void)unused;
@@ -234,10 +425,12 @@ extern "C" int64_t dst_adapter_tile_capacity(int64_t rows, int64_t bins, int til
   return 4 + 2 * (std::min(rows, dst::cdiv64(rows, tile) + bins) + 1);
 }
 
+static bool one_cluster(int64_t entries, int64_t bins) { return entries <= dst::CLUSTER_ENTRIES && bins <= dst::CLUSTER_BINS; }
+
 extern "C" size_t dst_adapter_plan_workspace_bytes(int64_t rows, int64_t n) {
   using namespace dst;
-  if (rows <= 0 || n <= 0 || (rows <= PLAN_ROWS && n < PLAN_BINS)) return 0;
-  return align16(rows * 4) + align16(rows * 8) + align16((n + 2) * 8) + align16(dst_sort_workspace_bytes(rows, n + 1));
+  if (rows <= SMALL || n <= 0 || one_cluster(rows, n + 1)) return 0;
+  return align16(rows * 8) + align16((n + 2) * 8) + align16(dst_sort_workspace_bytes(rows, n + 1));
 }
 
 extern "C" int dst_adapter_plan(const int32_t* offsets, const int32_t* slots, int64_t requests, int64_t rows, int64_t n, int tile,
@@ -249,37 +442,30 @@ extern "C" int dst_adapter_plan(const int32_t* offsets, const int32_t* slots, in
   if (!bin_offsets || !tiles || (rows > 0 && (!order || !bins)) || (requests > 0 && !slots)) return DST_ERR_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(tiles) & 7) != 0) return DST_ERR_ALIGNMENT;
   auto st = static_cast<cudaStream_t>(stream);
-  if (rows <= PLAN_ROWS && n < PLAN_BINS) {
-    const size_t smem = ((size_t)PLAN_WARPS * (n + 1) + 2 * (n + 2)) * 4 + (size_t)rows * 2;  // at most 168 KB
-    if (smem > 48 * 1024) DST_CUDA_TRY(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    plan_kernel<<<1, PLAN_THREADS, smem, st>>>(offsets, slots, requests, (int)rows, (int)n, tile, order, bins, bin_offsets, tiles);
-    DST_CUDA_TRY(cudaGetLastError());
-    return DST_OK;
-  }
-  if (rows == 0) {
-    DST_CUDA_TRY(cudaMemsetAsync(bin_offsets, 0, (size_t)(n + 2) * sizeof(int32_t), st));
-    DST_CUDA_TRY(cudaMemsetAsync(tiles, 0, 6 * sizeof(int32_t), st));  // no tile, the end at position 0
-    return DST_OK;
-  }
+  Plan a{};
+  a.offsets = offsets, a.slots = slots, a.requests = requests, a.entries = (int)rows, a.n = (int)n, a.tile = tile;
+  a.order = order, a.bins = bins, a.bin_offsets = bin_offsets, a.tiles = tiles;
+  if (rows <= (n < CLUSTER_BINS ? RANK_ROWS : SMALL)) return launch_small(a, st);
+  if (one_cluster(rows, n + 1)) return launch_cluster<false>(a, st);
   if (!workspace || workspace_bytes < dst_adapter_plan_workspace_bytes(rows, n)) return DST_ERR_BAD_ARG;
   char* w = static_cast<char*>(workspace);
-  int32_t* bin = reinterpret_cast<int32_t*>(w);
-  int64_t* order64 = reinterpret_cast<int64_t*>(w += align16(rows * 4));
+  int64_t* order64 = reinterpret_cast<int64_t*>(w);
   int64_t* offsets64 = reinterpret_cast<int64_t*>(w += align16(rows * 8));
-  bins_kernel<<<(unsigned)cdiv64(rows, 256), 256, 0, st>>>(offsets, slots, requests, rows, (int)n, bin);
+  bins_kernel<<<(unsigned)cdiv64(rows, 256), 256, 0, st>>>(offsets, slots, requests, rows, (int)n, bins);
   DST_CUDA_TRY(cudaGetLastError());
-  const int rc = sort_rows(bin, 1, rows, n + 1, order64, offsets64, nullptr, w + align16((n + 2) * 8), nullptr, st);
+  const int rc = sort_rows(bins, 1, rows, n + 1, order64, offsets64, nullptr, w + align16((n + 2) * 8), nullptr, st);
   if (rc != DST_OK) return rc;
-  lists_kernel<<<(unsigned)std::min<int64_t>(cdiv64(rows, PLAN_THREADS), 296), PLAN_THREADS, 0, st>>>(order64, offsets64, bin, rows, (int)n, tile,
-                                                                                                    order, bins, bin_offsets, tiles);
+  lists_kernel<<<(unsigned)std::min<int64_t>(cdiv64(rows, THREADS), 296), THREADS, 0, st>>>(order64, offsets64, rows, (int)n, tile, order,
+                                                                                          bin_offsets, tiles);
   DST_CUDA_TRY(cudaGetLastError());
   return DST_OK;
 }
 
 extern "C" size_t dst_adapter_plan_experts_workspace_bytes(int64_t pairs, int64_t E) {
   using namespace dst;
-  if (pairs <= 0 || E <= 0) return 0;
-  return align16(pairs * 4) + align16(pairs * 8) + align16(cdiv64(pairs, PLAN_THREADS) * 4) + align16(dst_sort_workspace_bytes(pairs, E));
+  if (pairs <= 0 || E <= 0 || pairs <= (E <= CLUSTER_BINS ? RANK_PAIRS : SMALL)) return 0;
+  if (one_cluster(pairs, E)) return align16(pairs * 4);
+  return align16(pairs * 4) + align16(pairs * 8) + align16(cdiv64(pairs, THREADS) * 4) + align16(dst_sort_workspace_bytes(pairs, E));
 }
 
 extern "C" int dst_adapter_plan_experts(const int32_t* ids, int64_t T, int top_k, int64_t E, const int32_t* order, const int32_t* bins, int64_t n,
@@ -292,14 +478,18 @@ extern "C" int dst_adapter_plan_experts(const int32_t* ids, int64_t T, int top_k
   if ((reinterpret_cast<uintptr_t>(tiles) & 7) != 0) return DST_ERR_ALIGNMENT;
   auto st = static_cast<cudaStream_t>(stream);
   const int64_t pairs = T * top_k;
-  if (pairs == 0) {
-    DST_CUDA_TRY(cudaMemsetAsync(tiles, 0, 6 * sizeof(int32_t), st));  // no tile, the end at position 0
-    DST_CUDA_TRY(cudaMemsetAsync(offsets, 0, (size_t)(E + 1) * sizeof(int64_t), st));
-    return DST_OK;
+  if (pairs > 0 && (!ids || !order || !bins || !pair_order || !x_rows)) return DST_ERR_BAD_ARG;
+  const size_t need = dst_adapter_plan_experts_workspace_bytes(pairs, E);
+  if (need && (!workspace || workspace_bytes < need)) return DST_ERR_BAD_ARG;
+  if (pairs <= SMALL || one_cluster(pairs, E)) {
+    const bool small = pairs <= (E <= CLUSTER_BINS ? RANK_PAIRS : SMALL);
+    Plan p{};
+    p.ids = ids, p.row_order = order, p.row_bins = bins, p.entries = (int)pairs, p.n = (int)n, p.k = top_k, p.E = (int)E, p.tile = tile;
+    p.pair_order = pair_order, p.expert_offsets = offsets, p.x_rows = x_rows, p.tiles = tiles, p.keys = static_cast<int32_t*>(workspace);
+    if (pairs == 0) p.ids = reinterpret_cast<const int32_t*>(tiles);  // not read: says that these are pairs
+    return small ? launch_small(p, st) : launch_cluster<true>(p, st);
   }
-  if (!ids || !order || !bins || !pair_order || !x_rows || !workspace || workspace_bytes < dst_adapter_plan_experts_workspace_bytes(pairs, E))
-    return DST_ERR_BAD_ARG;
-  const unsigned blocks = (unsigned)cdiv64(pairs, PLAN_THREADS);
+  const unsigned blocks = (unsigned)cdiv64(pairs, THREADS);
   char* w = static_cast<char*>(workspace);
   PairLists a{};
   int32_t* permuted = reinterpret_cast<int32_t*>(w);
@@ -313,8 +503,8 @@ extern "C" int dst_adapter_plan_experts(const int32_t* ids, int64_t T, int top_k
   pair_count_kernel<<<1, 1, 0, st>>>(offsets, (int)E, tiles);
   a.sorted = sorted, a.permuted = permuted, a.order = order, a.bins = bins, a.pairs = pairs, a.k = top_k, a.E = (int)E, a.n = (int)n, a.tile = tile;
   a.pair_order = pair_order, a.x_rows = x_rows, a.tiles = tiles;
-  pair_lists_kernel<false><<<blocks, PLAN_THREADS, 0, st>>>(a);
-  pair_lists_kernel<true><<<blocks, PLAN_THREADS, 0, st>>>(a);
+  pair_lists_kernel<false><<<blocks, THREADS, 0, st>>>(a);
+  pair_lists_kernel<true><<<blocks, THREADS, 0, st>>>(a);
   DST_CUDA_TRY(cudaGetLastError());
   return DST_OK;
 }

@@ -130,25 +130,32 @@ class B200Ops:
             raise ValueError(f"group_score must be one of {sorted(_lib.GROUP_SCORES)}, got {group_score!r}")
         if not logits.is_cuda:
             raise RuntimeError(kb._UNAVAILABLE + ": router logits are not on a CUDA device")
-        if logits.dtype not in kb._OUT:
-            logits = logits.float()
+        code = kb._OUT.get(logits.dtype)
+        if code is None:
+            logits, code = logits.float(), _lib.OUT_F32
         if logits.dim() != 2:
             raise RuntimeError("router logits are [tokens, experts]")
         T, E = logits.shape
-        if (E != 1 and logits.stride(1) != 1) or (T > 1 and logits.stride(0) < E):
-            logits = logits.contiguous()
+        stride, dev = E, logits.device
+        if not logits.is_contiguous():
+            if logits.stride(1) != 1 or logits.stride(0) < E:
+                logits = logits.contiguous()
+            stride = max(logits.stride(0), E)
+        p_bias = None
         if bias is not None:
-            bias = bias.to(device=logits.device, dtype=torch.float32).contiguous()
+            if bias.dtype is not torch.float32 or bias.device != dev or not bias.is_contiguous():
+                bias = bias.to(device=dev, dtype=torch.float32).contiguous()
             if bias.numel() != E:
                 raise ValueError("the gate bias holds one value per expert")
-        w = torch.empty(T, top_k, dtype=torch.float32, device=logits.device)
-        ids = torch.empty(T, top_k, dtype=torch.int32, device=logits.device)
-        with kb._guard(logits.device):
-            _lib.check(lib.dst_route_group_topk(logits.data_ptr(), kb._OUT[logits.dtype], max(logits.stride(0), E),
-                                                bias.data_ptr() if bias is not None else None, T, E, n_groups,
-                                                n_groups if topk_groups is None else topk_groups, _lib.GROUP_SCORES[group_score], top_k,
-                                                _lib.SCORE_FUNCS[score_func], gate_temp, 1 if renorm else 0, route_scale, w.data_ptr(),
-                                                ids.data_ptr(), kb._stream(logits)))
+            p_bias = bias.data_ptr()
+        w = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+        ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+        with kb._guard(dev):
+            rc = lib.dst_route_group_topk(logits.data_ptr(), code, stride, p_bias, T, E, n_groups, n_groups if topk_groups is None else topk_groups,
+                                          _lib.GROUP_SCORES[group_score], top_k, _lib.SCORE_FUNCS[score_func], gate_temp, 1 if renorm else 0,
+                                          route_scale, w.data_ptr(), ids.data_ptr(), kb._stream(logits))
+        if rc:
+            _lib.check(rc)
         return w, ids
 
     def sort(self, ids: torch.Tensor, n_experts: int):

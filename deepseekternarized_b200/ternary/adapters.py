@@ -12,6 +12,7 @@ and cleared in place, so captured graphs keep reading them. There is no CPU path
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 
 import torch
 
@@ -24,11 +25,34 @@ _EXPERT_TILE = 16
 
 
 def _int32(t: torch.Tensor, what: str) -> torch.Tensor:
+    if t.dtype is torch.int32 and t.is_cuda and t.is_contiguous():
+        return t
     if not t.is_cuda:
         raise RuntimeError(_UNAVAILABLE.format(what + " are"))
     if t.dtype not in (torch.int32, torch.int64):
         raise RuntimeError(f"{what} must be int32 or int64")
     return t.contiguous() if t.dtype == torch.int32 else t.clamp(-1, 0x7fffffff).to(torch.int32).contiguous()
+
+
+@lru_cache(4096)
+def _plan_sizes(n_rows: int, n_adapters: int):
+    """(tile, most tiles, first int32 of order / bins / offsets in the plan's buffer, workspace bytes) of a plan's sizes."""
+    if n_adapters < 1 or n_adapters > 4095 or n_rows < 0:
+        raise RuntimeError("a plan takes 1 to 4095 adapters")
+    lib = kb._require("auto")
+    tile = int(lib.dst_adapter_tile(n_rows))
+    at = int(lib.dst_adapter_tile_capacity(n_rows, n_adapters + 1, tile))
+    return tile, min(n_rows, -(-n_rows // tile) + n_adapters + 1), at, at + n_rows, at + 2 * n_rows, int(lib.dst_adapter_plan_workspace_bytes(n_rows, n_adapters))
+
+
+@lru_cache(4096)
+def _pair_sizes(pairs: int, n_adapters: int, n_experts: int):
+    """(most tiles, int64 words of the tile list, of all, workspace bytes) of an expert plan's sizes."""
+    lib = kb._require("auto")
+    bins = (n_adapters + 1) * n_experts
+    tiles = -(-int(lib.dst_adapter_tile_capacity(pairs, bins, _EXPERT_TILE)) // 2)
+    return min(pairs, -(-pairs // _EXPERT_TILE) + bins), tiles, pairs + n_experts + 1 + tiles + -(-pairs // 2), \
+        int(lib.dst_adapter_plan_experts_workspace_bytes(pairs, n_experts))
 
 
 class AdapterPlan:
@@ -56,29 +80,31 @@ class AdapterPlan:
         lib = kb._require("auto")
         slots = _int32(slots, "slots")
         dev = slots.device
+        p_offsets = None
         if offsets is not None:
             offsets = _int32(offsets, "offsets")
             if offsets.device != dev:
                 raise RuntimeError("offsets and slots must share one device")
-        if n_adapters < 1 or n_adapters > 4095 or n_rows < 0:
-            raise RuntimeError("a plan takes 1 to 4095 adapters")
-        self.n_rows, self.n_adapters, self.device = n_rows, n_adapters, dev
-        tile = self.tile = int(lib.dst_adapter_tile(n_rows))
-        self.max_tiles = min(n_rows, -(-n_rows // tile) + n_adapters + 1)
+            p_offsets = offsets.data_ptr()
+        tile, max_tiles, at_order, at_bins, at_offsets, ws_bytes = _plan_sizes(n_rows, n_adapters)
+        self.n_rows, self.n_adapters, self.tile, self.max_tiles, self.device = n_rows, n_adapters, tile, max_tiles, dev
         # one buffer: tiles, order, bins, offsets
-        at_order = int(lib.dst_adapter_tile_capacity(n_rows, n_adapters + 1, tile))
-        at_bins, at_offsets = at_order + n_rows, at_order + 2 * n_rows
         self._buf = torch.empty(at_offsets + n_adapters + 2, dtype=torch.int32, device=dev)
         self._at = at_order, at_bins, at_offsets
         base = self._buf.data_ptr()
-        ws_bytes = int(lib.dst_adapter_plan_workspace_bytes(n_rows, n_adapters))
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         with kb._guard(dev):
-            _lib.check(lib.dst_adapter_plan(offsets.data_ptr() if offsets is not None else None, slots.data_ptr(), slots.size(0), n_rows, n_adapters,
-                                            tile, base + 4 * at_order, base + 4 * at_bins, base + 4 * at_offsets, base,
-                                            ws.data_ptr() if ws is not None else None, ws_bytes, kb._stream(slots)))
-        self._c = _lib.AdapterRowsC(rows=base + 4 * at_order, x_rows=base + 4 * at_order, tiles=base, max_tiles=self.max_tiles, tile=tile)
-        self._ref = ctypes.byref(self._c)
+            _lib.check(lib.dst_adapter_plan(p_offsets, slots.data_ptr(), slots.size(0), n_rows, n_adapters, tile, base + 4 * at_order,
+                                            base + 4 * at_bins, base + 4 * at_offsets, base, ws.data_ptr() if ws is not None else None, ws_bytes,
+                                            kb._stream(slots)))
+        self._c = None
+
+    def _rows_c(self, pair_rows: bool):
+        """The C struct of these rows, made when a projection asks for it first."""
+        if self._c is None:
+            base = self._buf.data_ptr()
+            self._c = ctypes.byref(_lib.AdapterRowsC(base + 4 * self._at[0], base + 4 * self._at[0], base, self.max_tiles, self.tile))
+        return self._c
 
     @property
     def rows(self) -> torch.Tensor:
@@ -102,26 +128,45 @@ class ExpertPlan:
         lib = kb._require("auto")
         if ids.dim() != 2 or ids.size(0) != plan.n_rows or ids.size(1) < 1:
             raise RuntimeError("ids are [tokens, top_k] of the plan's rows")
-        if ids.is_cuda and ids.device != plan.device:
-            raise RuntimeError("ids and the plan must share one device")
         ids = _int32(ids, "expert ids")
+        if ids.device != plan.device:
+            raise RuntimeError("ids and the plan must share one device")
         T, k = ids.shape
         P, n, dev = T * k, plan.n_adapters, plan.device
         self.tokens, self.n_rows, self.n_adapters, self.n_experts, self.tile, self.device = T, P, n, n_experts, _EXPERT_TILE, dev
-        self.max_tiles = min(P, -(-P // _EXPERT_TILE) + (n + 1) * n_experts)
-        self.order = torch.empty(P, dtype=torch.int64, device=dev)
-        self.offsets = torch.empty(n_experts + 1, dtype=torch.int64, device=dev)
-        cap = int(lib.dst_adapter_tile_capacity(P, (n + 1) * n_experts, _EXPERT_TILE))
-        self._buf = torch.empty(cap + P, dtype=torch.int32, device=dev)
-        ws_bytes = int(lib.dst_adapter_plan_experts_workspace_bytes(P, n_experts))
-        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
+        self.max_tiles, tiles, words, ws_bytes = _pair_sizes(P, n, n_experts)
+        # one buffer of 64-bit words: order, offsets, tiles, x rows
+        self._buf = torch.empty(words, dtype=torch.int64, device=dev)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         base, src = self._buf.data_ptr(), plan._buf.data_ptr()
+        p_offsets = base + 8 * P
+        self._tiles = p_offsets + 8 * (n_experts + 1)
+        self._x_rows = self._tiles + 8 * tiles
         with kb._guard(dev):
             _lib.check(lib.dst_adapter_plan_experts(ids.data_ptr(), T, k, n_experts, src + 4 * plan._at[0], src + 4 * plan._at[1], n, _EXPERT_TILE,
-                                                    self.order.data_ptr(), self.offsets.data_ptr(), base + 4 * cap, base, ws.data_ptr(), ws_bytes,
-                                                    kb._stream(ids)))
-        self._pairs = _lib.AdapterRowsC(rows=None, x_rows=None, tiles=base, max_tiles=self.max_tiles, tile=_EXPERT_TILE)
-        self._tokens = _lib.AdapterRowsC(rows=None, x_rows=base + 4 * cap, tiles=base, max_tiles=self.max_tiles, tile=_EXPERT_TILE)
+                                                    base, p_offsets, self._x_rows, self._tiles, ws.data_ptr() if ws is not None else None,
+                                                    ws_bytes, kb._stream(ids)))
+        self._order = self._offsets = None
+        self._c = [None, None]
+
+    def _rows_c(self, pair_rows: bool):
+        """The C struct of the pairs with x rows of the tokens or of the pairs, made when a projection asks for it first."""
+        c = self._c[pair_rows]
+        if c is None:
+            c = self._c[pair_rows] = ctypes.byref(_lib.AdapterRowsC(None, None if pair_rows else self._x_rows, self._tiles, self.max_tiles, self.tile))
+        return c
+
+    @property
+    def order(self) -> torch.Tensor:
+        if self._order is None:
+            self._order = self._buf[:self.n_rows]
+        return self._order
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        if self._offsets is None:
+            self._offsets = self._buf[self.n_rows:self.n_rows + self.n_experts + 1]
+        return self._offsets
 
 
 class LowRankAdapters:
@@ -189,39 +234,53 @@ class LowRankAdapters:
         (``pair_rows``: one per pair too). Positions behind its last pair are not written."""
         if not x.is_cuda:
             raise RuntimeError(_UNAVAILABLE.format("activations are"))
-        pairs = isinstance(plan, ExpertPlan)
-        if pairs != (self.experts is not None) or plan.n_adapters != self.n_adapters or (pairs and plan.n_experts != self.experts):
+        pairs = type(plan) is ExpertPlan
+        if plan.n_adapters != self.n_adapters or pairs != (self.experts is not None) or (pairs and plan.n_experts != self.experts):
             raise RuntimeError("the plan was made for other adapters")
         if pair_rows and not pairs:
             raise RuntimeError("pair_rows goes with an expert plan")
-        if x.dtype != self.dtype:
+        if x.dtype is not self.dtype:
             raise TypeError(f"the adapters take {self.dtype} activations")
-        P = plan.n_rows
-        if x.dim() != 2 or x.size(1) != self.K or x.size(0) != (plan.tokens if pairs and not pair_rows else P):
+        P, N, K, dev = plan.n_rows, self.N, self.K, self.device
+        if x.shape != (plan.tokens if pairs and not pair_rows else P, K):
             raise RuntimeError("inconsistent adapter shapes")
-        x = _rows(x)
+        x_stride = K
+        if not x.is_contiguous():
+            x = _rows(x)
+            x_stride = max(x.stride(0), K)
+        p_base, base_code, base_stride = None, 0, N
         if base is not None:
-            if base.dim() != 2 or tuple(base.shape) != (P, self.N) or base.dtype not in kb._OUT:
+            base_code = kb._OUT.get(base.dtype)
+            if base_code is None or base.shape != (P, N):
                 raise RuntimeError("the base is float32, bf16 or fp16 [rows, N]")
-            base = _rows(base)
+            if base.device != dev:
+                raise RuntimeError("adapters, plan and tensors must share one device")
+            if not base.is_contiguous():
+                base = _rows(base)
+                base_stride = max(base.stride(0), N)
+            p_base = base.data_ptr()
+        out_stride = N
         if out is None:
-            out = torch.empty(P, self.N, dtype=out_dtype or (base.dtype if base is not None else x.dtype), device=x.device)
-        if out.dim() != 2 or tuple(out.shape) != (P, self.N) or out.dtype not in kb._OUT or (out_dtype is not None and out.dtype != out_dtype) \
-                or (P > 0 and out.stride(1) != 1) or (P > 1 and out.stride(0) < self.N):
+            out = torch.empty((P, N), dtype=out_dtype or (base.dtype if base is not None else x.dtype), device=dev)
+        elif out.shape != (P, N) or (out_dtype is not None and out.dtype != out_dtype) or out.device != dev \
+                or (P > 0 and out.stride(1) != 1 and N > 1) or (P > 1 and out.stride(0) < N):
             raise RuntimeError("the result is float32, bf16 or fp16 [rows, N]")
-        if not (self.device == plan.device == x.device == out.device) or (base is not None and base.device != x.device):
+        else:
+            out_stride = max(out.stride(0), N)
+        out_code = kb._OUT.get(out.dtype)
+        if out_code is None:
+            raise RuntimeError("the result is float32, bf16 or fp16 [rows, N]")
+        if x.device != dev or plan.device != dev:
             raise RuntimeError("adapters, plan and tensors must share one device")
-        if P == 0:
-            return out
-        c = plan._ref if not pairs else ctypes.byref(plan._pairs if pair_rows else plan._tokens)
-        with kb._guard(x.device):
-            _lib.check(kb._require("auto").dst_adapter_apply(
-                self._ref, c, x.data_ptr(), max(x.stride(0), self.K), base.data_ptr() if base is not None else None,
-                kb._OUT[base.dtype] if base is not None else 0, max(base.stride(0), self.N) if base is not None else self.N,
-                out.data_ptr(), kb._OUT[out.dtype], max(out.stride(0), self.N), kb._stream(x)))
+        if P:
+            with kb._guard(dev):
+                rc = kb._require("auto").dst_adapter_apply(self._ref, plan._rows_c(pair_rows), x.data_ptr(), x_stride, p_base, base_code, base_stride,
+                                                           out.data_ptr(), out_code, out_stride, kb._stream(x))
+            if rc:
+                _lib.check(rc)
         return out
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """Rows of neighbouring elements, one behind the other at any distance; anything else is copied."""
-    return t if t.stride(1) == 1 and (t.stride(0) >= t.size(1) or t.size(0) == 1) else t.contiguous()
+    return t if (t.stride(1) == 1 or t.size(1) == 1) and (t.stride(0) >= t.size(1) or t.size(0) == 1) else t.contiguous()
