@@ -29,6 +29,7 @@ ACT_BF16, ACT_F16, ACT_I8, ACT_F16_NORM = 0, 1, 2, 3
 ALGO_AUTO, ALGO_GENERIC, ALGO_DECODE, ALGO_PREFILL = 0, 1, 2, 3
 MAX_TERMS = 4
 MAX_PEERS = 16
+ADAPTER_TILE = 16
 LAYOUT_CANONICAL, LAYOUT_TILED = 0, 1
 SCORE_FUNCS = {"softmax": 0, "sigmoid": 1, "sqrtsoftplus": 2}
 GROUP_SCORES = {"max": 0, "top2": 1}
@@ -80,7 +81,7 @@ class AdaptersC(ctypes.Structure):
 class AdapterRowsC(ctypes.Structure):
     """``dst_adapter_rows`` of ``include/dst_b200.h``."""
 
-    _fields_ = [(name, ctypes.c_void_p) for name in ("rows", "x_rows", "tiles")] + [("max_tiles", ctypes.c_int64), ("tile", ctypes.c_int)]
+    _fields_ = [(name, ctypes.c_void_p) for name in ("rows", "x_rows", "tiles")] + [("max_tiles", ctypes.c_int64), ("positions", ctypes.c_int64), ("tile", ctypes.c_int)]
 
 
 _SIGNATURES = {
@@ -127,7 +128,6 @@ _SIGNATURES = {
     "dst_route_group_topk": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                                             ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int,
                                             ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
-    "dst_adapter_tile": (ctypes.c_int, [ctypes.c_int64]),
     "dst_adapter_tile_capacity": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
     "dst_adapter_plan_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
     "dst_adapter_plan": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
@@ -138,7 +138,9 @@ _SIGNATURES = {
                                                 ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                                 ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "dst_adapter_apply": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int,
-                                         ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p]),
+                                         ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t,
+                                         ctypes.c_void_p]),
+    "dst_adapter_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p, ctypes.c_void_p]),
     "dst_combine_add": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
                                        ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "dst_ep_combine_pull_add": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,

@@ -21,7 +21,7 @@ from ..kernels import ternary_b200 as kb
 
 _UNAVAILABLE = "the B200 adapters are unavailable: {} not on a CUDA device and this backend has no CPU path"
 _PADDED_RANKS = (16, 32, 64, 128)
-_EXPERT_TILE = 16
+_TILE = _lib.ADAPTER_TILE
 
 
 def _int32(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -36,13 +36,12 @@ def _int32(t: torch.Tensor, what: str) -> torch.Tensor:
 
 @lru_cache(4096)
 def _plan_sizes(n_rows: int, n_adapters: int):
-    """(tile, most tiles, first int32 of order / bins / offsets in the plan's buffer, workspace bytes) of a plan's sizes."""
+    """(most tiles, first int32 of order / bins / offsets in the plan's buffer, workspace bytes) of a plan's sizes."""
     if n_adapters < 1 or n_adapters > 4095 or n_rows < 0:
         raise RuntimeError("a plan takes 1 to 4095 adapters")
     lib = kb._require("auto")
-    tile = int(lib.dst_adapter_tile(n_rows))
-    at = int(lib.dst_adapter_tile_capacity(n_rows, n_adapters + 1, tile))
-    return tile, min(n_rows, -(-n_rows // tile) + n_adapters + 1), at, at + n_rows, at + 2 * n_rows, int(lib.dst_adapter_plan_workspace_bytes(n_rows, n_adapters))
+    at = int(lib.dst_adapter_tile_capacity(n_rows, n_adapters + 1, _TILE))
+    return min(n_rows, -(-n_rows // _TILE) + n_adapters + 1), at, at + n_rows, at + 2 * n_rows, int(lib.dst_adapter_plan_workspace_bytes(n_rows, n_adapters))
 
 
 @lru_cache(4096)
@@ -50,8 +49,8 @@ def _pair_sizes(pairs: int, n_adapters: int, n_experts: int):
     """(most tiles, int64 words of the tile list, of all, workspace bytes) of an expert plan's sizes."""
     lib = kb._require("auto")
     bins = (n_adapters + 1) * n_experts
-    tiles = -(-int(lib.dst_adapter_tile_capacity(pairs, bins, _EXPERT_TILE)) // 2)
-    return min(pairs, -(-pairs // _EXPERT_TILE) + bins), tiles, pairs + n_experts + 1 + tiles + -(-pairs // 2), \
+    tiles = -(-int(lib.dst_adapter_tile_capacity(pairs, bins, _TILE)) // 2)
+    return min(pairs, -(-pairs // _TILE) + bins), tiles, pairs + n_experts + 1 + tiles + -(-pairs // 2), \
         int(lib.dst_adapter_plan_experts_workspace_bytes(pairs, n_experts))
 
 
@@ -86,15 +85,15 @@ class AdapterPlan:
             if offsets.device != dev:
                 raise RuntimeError("offsets and slots must share one device")
             p_offsets = offsets.data_ptr()
-        tile, max_tiles, at_order, at_bins, at_offsets, ws_bytes = _plan_sizes(n_rows, n_adapters)
-        self.n_rows, self.n_adapters, self.tile, self.max_tiles, self.device = n_rows, n_adapters, tile, max_tiles, dev
+        max_tiles, at_order, at_bins, at_offsets, ws_bytes = _plan_sizes(n_rows, n_adapters)
+        self.n_rows, self.n_adapters, self.max_tiles, self.device = n_rows, n_adapters, max_tiles, dev
         # one buffer: tiles, order, bins, offsets
         self._buf = torch.empty(at_offsets + n_adapters + 2, dtype=torch.int32, device=dev)
         self._at = at_order, at_bins, at_offsets
         base = self._buf.data_ptr()
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         with kb._guard(dev):
-            _lib.check(lib.dst_adapter_plan(p_offsets, slots.data_ptr(), slots.size(0), n_rows, n_adapters, tile, base + 4 * at_order,
+            _lib.check(lib.dst_adapter_plan(p_offsets, slots.data_ptr(), slots.size(0), n_rows, n_adapters, _TILE, base + 4 * at_order,
                                             base + 4 * at_bins, base + 4 * at_offsets, base, ws.data_ptr() if ws is not None else None, ws_bytes,
                                             kb._stream(slots)))
         self._c = None
@@ -103,7 +102,7 @@ class AdapterPlan:
         """The C struct of these rows, made when a projection asks for it first."""
         if self._c is None:
             base = self._buf.data_ptr()
-            self._c = ctypes.byref(_lib.AdapterRowsC(base + 4 * self._at[0], base + 4 * self._at[0], base, self.max_tiles, self.tile))
+            self._c = ctypes.byref(_lib.AdapterRowsC(base + 4 * self._at[0], base + 4 * self._at[0], base, self.max_tiles, self.n_rows, _TILE))
         return self._c
 
     @property
@@ -133,7 +132,7 @@ class ExpertPlan:
             raise RuntimeError("ids and the plan must share one device")
         T, k = ids.shape
         P, n, dev = T * k, plan.n_adapters, plan.device
-        self.tokens, self.n_rows, self.n_adapters, self.n_experts, self.tile, self.device = T, P, n, n_experts, _EXPERT_TILE, dev
+        self.tokens, self.n_rows, self.n_adapters, self.n_experts, self.device = T, P, n, n_experts, dev
         self.max_tiles, tiles, words, ws_bytes = _pair_sizes(P, n, n_experts)
         # one buffer of 64-bit words: order, offsets, tiles, x rows
         self._buf = torch.empty(words, dtype=torch.int64, device=dev)
@@ -143,7 +142,7 @@ class ExpertPlan:
         self._tiles = p_offsets + 8 * (n_experts + 1)
         self._x_rows = self._tiles + 8 * tiles
         with kb._guard(dev):
-            _lib.check(lib.dst_adapter_plan_experts(ids.data_ptr(), T, k, n_experts, src + 4 * plan._at[0], src + 4 * plan._at[1], n, _EXPERT_TILE,
+            _lib.check(lib.dst_adapter_plan_experts(ids.data_ptr(), T, k, n_experts, src + 4 * plan._at[0], src + 4 * plan._at[1], n, _TILE,
                                                     base, p_offsets, self._x_rows, self._tiles, ws.data_ptr() if ws is not None else None,
                                                     ws_bytes, kb._stream(ids)))
         self._order = self._offsets = None
@@ -153,7 +152,7 @@ class ExpertPlan:
         """The C struct of the pairs with x rows of the tokens or of the pairs, made when a projection asks for it first."""
         c = self._c[pair_rows]
         if c is None:
-            c = self._c[pair_rows] = ctypes.byref(_lib.AdapterRowsC(None, None if pair_rows else self._x_rows, self._tiles, self.max_tiles, self.tile))
+            c = self._c[pair_rows] = ctypes.byref(_lib.AdapterRowsC(None, None if pair_rows else self._x_rows, self._tiles, self.max_tiles, self.n_rows, _TILE))
         return c
 
     @property
@@ -200,6 +199,7 @@ class LowRankAdapters:
         self._c = _lib.AdaptersC(a=self._a.data_ptr(), b=self._b.data_ptr(), scale=self._scale.data_ptr(), ranks=self._ranks.data_ptr(),
                                  matrices_per_slot=E, K=K, K_padded=Kp, N=N, rank_padded=self.rank_padded, parts=parts, dtype=kb._ACT[dtype])
         self._ref = ctypes.byref(self._c)
+        self._ws_bytes = {}
 
     def load(self, slot: int, A: torch.Tensor, B: torch.Tensor, scale: float = 1.0) -> None:
         """Put an adapter into ``slot``: A [parts * r, K], B [N, r] (with ``experts``: [experts, ...] each), r <= ``rank``."""
@@ -273,9 +273,15 @@ class LowRankAdapters:
         if x.device != dev or plan.device != dev:
             raise RuntimeError("adapters, plan and tensors must share one device")
         if P:
+            c = plan._rows_c(pair_rows)
+            sizes = plan.max_tiles, P
+            ws_bytes = self._ws_bytes.get(sizes)
+            if ws_bytes is None:  # by sizes alone
+                ws_bytes = self._ws_bytes[sizes] = int(kb._require("auto").dst_adapter_workspace_bytes(self._ref, c))
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
             with kb._guard(dev):
-                rc = kb._require("auto").dst_adapter_apply(self._ref, plan._rows_c(pair_rows), x.data_ptr(), x_stride, p_base, base_code, base_stride,
-                                                           out.data_ptr(), out_code, out_stride, kb._stream(x))
+                rc = kb._require("auto").dst_adapter_apply(self._ref, c, x.data_ptr(), x_stride, p_base, base_code, base_stride, out.data_ptr(), out_code,
+                                                           out_stride, ws.data_ptr() if ws is not None else None, ws_bytes, kb._stream(x))
             if rc:
                 _lib.check(rc)
         return out

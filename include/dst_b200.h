@@ -300,7 +300,7 @@ int dst_moe_layer(const void* x_bf16, const float* weights, const int32_t* ids, 
  * and the combine take as order and offsets. x_rows [T * top_k] = the position's token. tiles
  * [dst_adapter_tile_capacity(T * top_k, (n + 1) * E, tile)]: matrix adapter * E + expert. E <= 4096.
  */
-int dst_adapter_tile(int64_t rows); /* the tile height that suits a plan of so many rows: 16, 32 or 64 */
+enum { DST_ADAPTER_TILE = 16 }; /* the rows of a tile that dst_adapter_apply takes */
 int64_t dst_adapter_tile_capacity(int64_t rows, int64_t bins, int tile);
 size_t dst_adapter_plan_workspace_bytes(int64_t rows, int64_t n);
 int dst_adapter_plan(const int32_t* offsets, const int32_t* slots, int64_t requests, int64_t rows, int64_t n, int tile, int32_t* order,
@@ -319,7 +319,8 @@ int dst_adapter_plan_experts(const int32_t* ids, int64_t T, int top_k, int64_t E
  * the rank ranks[a] <= rank_padded; what lies behind it is finite and counts for nothing (rank 0: the base alone).
  * rank_padded 16, 32, 64 or 128; parts 1 or 2 with parts * rank_padded <= 128; K_padded a multiple of 32.
  * rows / x_rows: base / out row and x row of a position (NULL: the position). base (DST_OUT_* type) may be NULL (zeros) or the
- * same rows as out; x may not overlap out. Strides in elements.
+ * same rows as out; x may not overlap out. Strides in elements. positions: rows of the plan (pairs of a layer). Workspace (16-byte
+ * aligned): dst_adapter_workspace_bytes, by sizes and rank_padded, parts, tile alone; 0 for few tiles.
  */
 typedef struct dst_adapters {
   const void* a;
@@ -333,11 +334,13 @@ typedef struct dst_adapter_rows {
   const int32_t* rows;
   const int32_t* x_rows;
   const int32_t* tiles;
-  int64_t max_tiles;
+  int64_t max_tiles, positions;
   int tile;
 } dst_adapter_rows;
+size_t dst_adapter_workspace_bytes(const dst_adapters* w, const dst_adapter_rows* plan);
 int dst_adapter_apply(const dst_adapters* w, const dst_adapter_rows* plan, const void* x, int64_t x_stride, const void* base, int base_dtype,
-                      int64_t base_stride, void* out, int out_dtype, int64_t out_stride, dst_stream_t stream);
+                      int64_t base_stride, void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                      dst_stream_t stream);
 
 /* The same with one more bf16 row per token added in fp32 after the experts' rows and before the cast: the shared
  * expert's output, `y += self.swiglu(L.shared, x)` of boilerplate/engine/model.py:421. add_bf16 [T, hidden] or NULL.
