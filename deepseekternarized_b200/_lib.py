@@ -16,7 +16,8 @@ from pathlib import Path
 CSRC = Path(__file__).resolve().parent / "csrc"
 LIB_PATH = CSRC / "libdst_b200.so"
 SOURCES = ["api.cu", "format_kernels.cu", "layout_kernels.cu", "gemm_generic.cu", "gemm_decode.cu", "gemm_decode_tq1.cu", "gemm_prefill.cu", "ep_kernels.cu",
-           "moe_kernels.cu", "moe_layer.cu", "route_group.cu", "adapter_plan.cu", "adapter_gemm.cu"]
+           "moe_kernels.cu", "moe_layer.cu", "route_group.cu", "adapter_plan.cu", "adapter_gemm.cu",
+           "adapter_gemm_bf16.cu", "adapter_gemm_f16.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-shared",
               "-Xcompiler", "-fPIC"]
 
@@ -29,7 +30,6 @@ ACT_BF16, ACT_F16, ACT_I8, ACT_F16_NORM = 0, 1, 2, 3
 ALGO_AUTO, ALGO_GENERIC, ALGO_DECODE, ALGO_PREFILL = 0, 1, 2, 3
 MAX_TERMS = 4
 MAX_PEERS = 16
-ADAPTER_TILE = 16
 LAYOUT_CANONICAL, LAYOUT_TILED = 0, 1
 SCORE_FUNCS = {"softmax": 0, "sigmoid": 1, "sqrtsoftplus": 2}
 GROUP_SCORES = {"max": 0, "top2": 1}
@@ -128,6 +128,7 @@ _SIGNATURES = {
     "dst_route_group_topk": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                                             ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int,
                                             ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "dst_adapter_tile": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64]),
     "dst_adapter_tile_capacity": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
     "dst_adapter_plan_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
     "dst_adapter_plan": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,

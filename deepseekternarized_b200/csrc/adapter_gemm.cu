@@ -1,1014 +1,57 @@
-// Low-rank adapters of many requests beside a projection:
-//
-//   out[r, :] = round( base[r, :] + scale_a * B_m (A_m x[x(r), :]) )      rows of an adapter a with matrices m
-//   out[r, :] = round( base[r, :] )                                       rows without one
-//
-// A_m [parts * rank, K], B_m [N, rank]: part p of the output's N / parts columns takes its own rank rows of A (the gate and up
-// matrices of an expert stacked, projections that share their input). h = A x is a sum of exact 16-bit products in fp32; it is
-// split into 16-bit pieces (bf16: two for 16-bit outputs, three for float32 ones, 2^-17 and 2^-25 of h; fp16: two, 2^-22, after a
-// power of two per row that keeps h in range), so that B h runs on the matrix instructions too without a rounding of h that the
-// result would show. base is added in fp32 and the sum rounded once.
-//
-// Two forms. Few tiles (decoding): a tile belongs to a cluster of CTAs, which share K for h, add their parts through the cluster's
-// shared memory and share the N columns after that: one launch, and latency is what counts. Many tiles: one kernel for h (its parts
-// go through a workspace), one for the columns, which starts early and has its first loads on the way when h is there; their
-// warps depend on nobody, so that loads never stop for a barrier, and memory traffic is what counts. Sums are added in a fixed order
-// in both: results do not depend on scheduling.
-#include <cooperative_groups.h>
-
+// C-ABI entry points of the low-rank adapters: argument checks and how a call is cut.
 #include <algorithm>
-#include <cstdlib>
 
-#include "dst_common.cuh"
+#include "adapter_call.cuh"
 
 namespace dst {
 namespace {
 
-namespace cg = cooperative_groups;
-
-struct AdapterCall {
-  const void* x;
-  int64_t x_stride;
-  const int32_t *x_rows, *rows, *tiles;  // x row and base / out row of a position; null: the position itself
-  const uint16_t *a, *b;
-  const float* scale;
-  const int32_t* ranks;
-  int64_t per_slot;  // matrices of one adapter
-  int64_t K, Kp, Np; // Kp: columns of A as stored; Np: columns of a part
-  int parts;
-  const void* base;
-  int64_t base_stride, out_stride;
-  void* out;
-  int base_dtype, out_dtype;  // DST_OUT_*; base null: zeros
-  int ctas, splits;           // of a cluster; of K (h) or of the columns between the CTAs of a tile
-  float* h;                   // [splits of K][positions][rows of A]
-  int64_t positions;
-  int k_splits, share;
-  int kind;                   // base and result of the fast forms: 0 float32 / 16 bits, 1 float32 / float32, 2 16 / 16, 3 none / 16; -1: others
-  int x_vec;                  // rows of x can be read eight values at a time
-};
-
-__device__ __forceinline__ void mma16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, __nv_bfloat16) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, __half) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// Eight 16-bit values of a row at element i of n, zeros behind its end
-__device__ __forceinline__ uint4 load8(const uint16_t* p, int64_t i, int64_t n, bool vec) {
-  if (vec && i + 8 <= n) return *reinterpret_cast<const uint4*>(p + i);
-  uint32_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t lo = i + 2 * j < n ? p[i + 2 * j] : 0u, hi = i + 2 * j + 1 < n ? p[i + 2 * j + 1] : 0u;
-    w[j] = lo | (hi << 16);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-__device__ __forceinline__ float to_float(uint16_t v, __nv_bfloat16) { return __uint_as_float((uint32_t)v << 16); }
-__device__ __forceinline__ float to_float(uint16_t v, __half) { return __half2float(__ushort_as_half(v)); }
-
-// The nearest 16-bit value below infinity in magnitude where v is finite, and what is left of v
-__device__ __forceinline__ uint16_t piece(float& v, __nv_bfloat16) {
-  const uint16_t h = __bfloat16_as_ushort(__float2bfloat16_rn(v));
-  v = isfinite(v) ? v - __uint_as_float((uint32_t)h << 16) : 0.f;
-  return h;
-}
-__device__ __forceinline__ uint16_t piece(float& v, __half) {
-  const float c = isfinite(v) ? fminf(fmaxf(v, -65504.f), 65504.f) : v;
-  const uint16_t h = __half_as_ushort(__float2half_rn(c));
-  v = isfinite(v) ? v - __half2float(__ushort_as_half(h)) : 0.f;
-  return h;
-}
-
-__device__ __forceinline__ float element(const void* p, int64_t i, int dtype) {
-  if (dtype == DST_OUT_F32) return static_cast<const float*>(p)[i];
-  if (dtype == DST_OUT_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  return __half2float(static_cast<const __half*>(p)[i]);
-}
-
-// Four values of a row and their sum with what `base` holds of it
-template <typename T>
-__device__ __forceinline__ uint2 pack4(const float* v) {
-  uint32_t w[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-      w[j] = *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-      const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-      w[j] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-  }
-  return make_uint2(w[0], w[1]);
-}
-
-// base + v for up to four neighbouring columns, of any types and alignment
-__device__ __forceinline__ void finish_single(const AdapterCall& c, int64_t row, int64_t col, int n, const float* v) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (j < n) {
-      const int64_t bi = row * c.base_stride + col + j, oi = row * c.out_stride + col + j;
-      const float r = c.base ? v[j] + element(c.base, bi, c.base_dtype) : v[j];
-      if (c.out_dtype == DST_OUT_F32) static_cast<float*>(c.out)[oi] = r;
-      else if (c.out_dtype == DST_OUT_BF16) static_cast<__nv_bfloat16*>(c.out)[oi] = __float2bfloat16_rn(r);
-      else static_cast<__half*>(c.out)[oi] = __float2half_rn(r);
-    }
-}
-
-// Asynchronous copies into a lane's own slots: no other thread reads them, so waiting for the lane's own groups is enough. A slot
-// is refilled after the instructions that used its values.
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {  // the rest of the 16 are zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copy8(uint32_t to, const void* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
-}
-__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint4 slot(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-  return v;
-}
-
-constexpr int WARPS = 8, MAX_CTAS = 8;
-constexpr int XS = 4, BS = 3;  // steps of x and of base on the way
-
-// RP: rank as stored (16, 32, 64 or 128), P: parts. The warps share K first and the columns then.
-template <typename T, int RP, int P>
-struct Shape {
-  static constexpr int R = RP * P, NT = R / 8, HS = R + 8;  // HS: row stride of the pieces of h, shifted banks
-  static constexpr int ROWS = 16, KW = WARPS;
-  static constexpr int XPART = XS * 1024 > 16 * R * 4 ? XS * 1024 : 16 * R * 4;  // bytes of a warp: steps of x, then its part of h
-  static constexpr int BPART = BS * 2048;                                        // steps of base: 16 rows of 32 columns
-  static constexpr int BASE = WARPS * XPART, PIECES = BASE + WARPS * BPART, SMEM = PIECES + 3 * ROWS * HS * 2;
-};
-
-// What a step of the second product meets: base float32 or of the 16-bit type or none, the result of the 16-bit type or float32
-enum { BASE_F32, BASE_T, BASE_NONE };
-template <int V>
-using Int = std::integral_constant<int, V>;
-
-template <typename T, int RP, int P>
-__global__ void __launch_bounds__(WARPS * 32, RP* P <= 64 ? 2 : 1) adapter_kernel(const AdapterCall c) {
-  using S = Shape<T, RP, P>;
-  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
-  constexpr int R = S::R, NT = S::NT, HS = S::HS, ROWS = S::ROWS, KW = S::KW, KB = RP == 16 ? 1 : RP / 32;
-  extern __shared__ __align__(16) char smem[];
-  uint16_t* pieces = reinterpret_cast<uint16_t*>(smem + S::PIECES);  // [3][ROWS][HS]
-  __shared__ float factor[ROWS];
-  const cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
-  const int tile = (int)(blockIdx.x / ctas);
-  if (tile >= c.tiles[0]) return;
-  const int2* list = reinterpret_cast<const int2*>(c.tiles + 4);
-  const int2 head = list[tile];
-  const int first = head.x, matrix = head.y, rows = min(list[tile + 1].x - first, ROWS);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
-  const int worker = cta * KW + warp, workers = ctas * KW;
-  const int ra = g, rb = g + 8;  // the lane's two rows of the tile
-  const bool va = ra < rows, vb = rb < rows;
-  const int pa = first + (va ? ra : 0), pb = first + (vb ? rb : 0);
-
-  // A of the warp's first step, before anything that depends on the rows
-  const uint16_t* a = c.a + (int64_t)(matrix < 0 ? 0 : matrix) * R * c.Kp + g * 32 + q * 8;
-  const int k_steps = matrix < 0 ? 0 : (int)(c.Kp / 32);
-  uint4 aw[NT];
-  const auto load_a = [&](int step, uint4 (&w)[NT]) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(a + (int64_t)step * (R * 32) + i * 256));
-  };
-  if (worker < k_steps) load_a(worker, aw);
-
-  // Steps of 32 columns, those of the second part behind those of the first. A lane has four neighbouring columns and the four 16
-  // further on: quads of lanes then read and write whole 32-byte sectors whatever the types.
-  const int Np = (int)c.Np, N = Np * P, per_part = (Np + 31) / 32, steps = per_part * P;
-  const auto column = [&](int step) { return step * 32 + (P == 2 && step >= per_part ? Np - per_part * 32 : 0); };
-  const auto behind = [&](int step, int col) { return (P == 2 && step < per_part ? Np : N) - col; };
-  const int64_t oa = c.rows ? c.rows[pa] : pa, ob = c.rows ? c.rows[pb] : pb;
-  const uint32_t base_slots = (uint32_t)__cvta_generic_to_shared(smem + S::BASE + warp * S::BPART) + lane * 16;
-  const int es = c.base_dtype == DST_OUT_F32 ? 4 : 2;
-  const char* base_a = static_cast<const char*>(c.base) + (oa * c.base_stride + 4 * q) * es;
-  const char* base_b = static_cast<const char*>(c.base) + (ob * c.base_stride + 4 * q) * es;
-  const int kind = c.kind;  // of what the fast form covers, else -1
-  const auto fetch_base = [&](auto base_kind, int step, int stage) {
-    if (decltype(base_kind)::value != BASE_NONE && step < steps) {
-      constexpr int ES = decltype(base_kind)::value == BASE_F32 ? 4 : 2;
-      const int col = column(step), left = behind(step, col) - 4 * q;
-      const char *fa = base_a + (int64_t)col * ES, *fb = base_b + (int64_t)col * ES;
-      const uint32_t to = base_slots + stage * 2048;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (left > 16 * i) {
-          if constexpr (ES == 4) {
-            if (va) copy16(to + i * 512, fa + 16 * ES * i, 16);
-            if (vb) copy16(to + 1024 + i * 512, fb + 16 * ES * i, 16);
-          } else {
-            if (va) copy8(to + i * 512, fa + 16 * ES * i);
-            if (vb) copy8(to + 1024 + i * 512, fb + 16 * ES * i);
-          }
-        }
-    }
-    commit();
-  };
-#pragma unroll
-  for (int s = 0; s < BS; ++s) {
-    if (kind == 0 || kind == 1) fetch_base(Int<BASE_F32>(), worker + s * workers, s);
-    else if (kind == 2) fetch_base(Int<BASE_T>(), worker + s * workers, s);
-  }
-  // B of a step. The eight rows of instruction j are columns 16 (j / 2) + 4 (g / 2) + 2 (j % 2) + g % 2, which gives a lane its
-  // own. Up to 31 rows behind the part's last one are read and not used.
-  const uint16_t* b = c.b + ((int64_t)(matrix < 0 ? 0 : matrix) * N + 4 * (g >> 1) + (g & 1)) * RP + q * (RP == 16 ? 4 : 8);
-  uint4 bw[KB][4];
-  const auto load_b = [&](int step, uint4 (&w)[KB][4]) {
-    if (matrix < 0 || step >= steps) return;
-    const uint16_t* p = b + (int64_t)column(step) * RP;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint16_t* br = p + (16 * (j >> 1) + 2 * (j & 1)) * RP;
-      if constexpr (RP == 16) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(br));
-        w[0][j].x = v.x, w[0][j].y = v.y;
-      } else {
-#pragma unroll
-        for (int k = 0; k < KB; ++k) w[k][j] = __ldg(reinterpret_cast<const uint4*>(br + k * 32));
-      }
-    }
-  };
-  constexpr bool EARLY_B = RP <= 32 && R <= 64;  // the first step's B before anything is waited for, where registers allow
-  if (EARLY_B) load_b(worker, bw);
-
-  if (matrix >= 0) {
-    // h: the warp's share of K, 32 values a step; a lane's eight neighbouring values feed two instructions (the order of k
-    // inside a step is the same for both operands, so it does not matter). A is stored step by step.
-    float acc[NT][4];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-    const uint16_t* xa = static_cast<const uint16_t*>(c.x) + (c.x_rows ? c.x_rows[pa] : pa) * c.x_stride + q * 8;
-    const uint16_t* xb = static_cast<const uint16_t*>(c.x) + (c.x_rows ? c.x_rows[pb] : pb) * c.x_stride + q * 8;
-    const uint32_t x_slots = (uint32_t)__cvta_generic_to_shared(smem + warp * S::XPART) + lane * 16;
-    const int K = (int)c.K;
-    const int full_a = va ? 16 : 0, full_b = vb ? 16 : 0;
-    const auto fetch_x = [&](int step, int stage) {
-      const uint32_t to = x_slots + stage * 1024;
-      if (step < k_steps) {
-        const int k = step * 32;
-        if (c.x_vec) {
-          const bool whole = k + 32 <= K;
-          const int bytes = whole ? 16 : min(16, max(0, (K - k - q * 8) * 2));
-          const int at = bytes > 0 ? k : 0;  // a copy of nothing still wants an address
-          copy16(to, xa + at, min(bytes, full_a));
-          copy16(to + 512, xb + at, min(bytes, full_b));
-        } else {
-          const uint4 u = va ? load8(xa, k, K - q * 8, false) : make_uint4(0, 0, 0, 0);
-          const uint4 v = vb ? load8(xb, k, K - q * 8, false) : make_uint4(0, 0, 0, 0);
-          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
-          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + 512), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-        }
-      }
-      commit();
-    };
-#pragma unroll
-    for (int s = 0; s < XS; ++s) fetch_x(worker + s * workers, s);
-    int stage = 0;
-    for (int step = worker; step < k_steps; step += workers) {
-      uint4 an[NT];
-      if (R <= 64 && step + workers < k_steps) load_a(step + workers, an);
-      wait_but<XS - 1>();
-      const uint4 u = slot(x_slots + stage * 1024), v = slot(x_slots + stage * 1024 + 512);
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        mma16(acc[i], u.x, v.x, u.y, v.y, aw[i].x, aw[i].y, T());
-        mma16(acc[i], u.z, v.z, u.w, v.w, aw[i].z, aw[i].w, T());
-      }
-      fetch_x(step + XS * workers, stage);
-      stage = (stage + 1) % XS;
-      if (R <= 64) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) aw[i] = an[i];
-      } else if (step + workers < k_steps) {
-        load_a(step + workers, aw);
-      }
-    }
-    if (!EARLY_B) load_b(worker, bw);  // on the way while the parts of h are added up
-    float* mine = reinterpret_cast<float*>(smem + warp * S::XPART);  // over the warp's own x, which is used up
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      *reinterpret_cast<float2*>(mine + g * R + i * 8 + 2 * q) = make_float2(acc[i][0], acc[i][1]);
-      *reinterpret_cast<float2*>(mine + (g + 8) * R + i * 8 + 2 * q) = make_float2(acc[i][2], acc[i][3]);
-    }
-    float* parts = reinterpret_cast<float*>(smem);
-    __syncthreads();
-    {
-      for (int i = tid * 4; i < ROWS * R; i += WARPS * 32 * 4) {
-        float4 s = *reinterpret_cast<float4*>(parts + i);
-#pragma unroll
-        for (int w = 1; w < KW; ++w) {
-          const float4 o = *reinterpret_cast<float4*>(parts + w * (S::XPART / 4) + i);
-          s.x += o.x, s.y += o.y, s.z += o.z, s.w += o.w;
-        }
-        *reinterpret_cast<float4*>(parts + i) = s;
-      }
-    }
-    cluster.sync();
-    // h of all CTAs, times the adapter's scale, in pieces: four neighbouring values a thread
-    const float scale = c.scale[matrix / c.per_slot];
-    const int rank = c.ranks[matrix / c.per_slot];
-    const int n_pieces = BF && (c.out_dtype == DST_OUT_F32 || kind < 0) ? 3 : 2;
-    const float* from[MAX_CTAS];
-#pragma unroll
-    for (int i = 0; i < MAX_CTAS; ++i) from[i] = cluster.map_shared_rank(parts, i < ctas ? i : 0);
-    for (int i = tid * 4; i < ROWS * R; i += WARPS * 32 * 4) {
-      const int row = i / R, col = i % R;
-      float4 o[MAX_CTAS];
-#pragma unroll
-      for (int k = 0; k < MAX_CTAS; ++k) o[k] = k < ctas ? *reinterpret_cast<const float4*>(from[k] + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-      float h[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < MAX_CTAS; ++k) h[0] += o[k].x, h[1] += o[k].y, h[2] += o[k].z, h[3] += o[k].w;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) h[j] = (col + j) % RP < rank ? h[j] * scale : 0.f;
-      if (!BF) {  // a row is R / 4 lanes of a warp
-        float big = fmaxf(fmaxf(fabsf(h[0]), fabsf(h[1])), fmaxf(fabsf(h[2]), fabsf(h[3])));
-#pragma unroll
-        for (int off = R / 8; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-        int ex = 0;
-        if (big > 0.f && isfinite(big)) {
-          (void)frexpf(big, &ex);
-          ex -= 8;  // the largest in [128, 256)
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = ldexpf(h[j], -ex);
-        if (col == 0) factor[row] = ldexpf(1.f, ex);
-      }
-#pragma unroll
-      for (int p = 0; p < 3; ++p)
-        if (p < n_pieces) {
-          const uint32_t h0 = piece(h[0], T()), h1 = piece(h[1], T()), h2 = piece(h[2], T()), h3 = piece(h[3], T());
-          *reinterpret_cast<uint2*>(pieces + (p * ROWS + row) * HS + col) = make_uint2(h0 | (h1 << 16), h2 | (h3 << 16));
-        }
-    }
-    cluster.sync();  // also: every CTA has read the others' parts
-  }
-
-  const float fa = !BF && matrix >= 0 ? factor[ra] : 1.f, fb = !BF && matrix >= 0 ? factor[rb] : 1.f;
-  // d = the pieces of h times B of a step (NP pieces)
-  const auto product = [&](auto np, int part, float (&d)[4][4]) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.f;
-    if (matrix < 0) return;
-#pragma unroll
-    for (int p = 0; p < decltype(np)::value; ++p) {
-      const uint16_t* ha = pieces + (p * ROWS + ra) * HS + part * RP;
-      const uint16_t* hb = pieces + (p * ROWS + rb) * HS + part * RP;
-      if constexpr (RP == 16) {
-        const uint2 u = *reinterpret_cast<const uint2*>(ha + q * 4), v = *reinterpret_cast<const uint2*>(hb + q * 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) mma16(d[j], u.x, v.x, u.y, v.y, bw[0][j].x, bw[0][j].y, T());
-      } else {
-#pragma unroll
-        for (int k = 0; k < KB; ++k) {
-          const uint4 u = *reinterpret_cast<const uint4*>(ha + k * 32 + q * 8), v = *reinterpret_cast<const uint4*>(hb + k * 32 + q * 8);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            mma16(d[j], u.x, v.x, u.y, v.y, bw[k][j].x, bw[k][j].y, T());
-            mma16(d[j], u.z, v.z, u.w, v.w, bw[k][j].z, bw[k][j].w, T());
-          }
-        }
-      }
-    }
-    if (!BF) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) d[j][0] *= fa, d[j][1] *= fa, d[j][2] *= fb, d[j][3] *= fb;
-    }
-  };
-  const auto next_b = [&](const uint4 (&w)[KB][4]) {
-#pragma unroll
-    for (int k = 0; k < KB; ++k)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) bw[k][j] = w[k][j];
-  };
-  const auto columns = [&](auto base_kind, auto out_f32) {
-    constexpr int BK = decltype(base_kind)::value;
-    constexpr bool OF = decltype(out_f32)::value != 0;
-    char* out_a = static_cast<char*>(c.out) + (oa * c.out_stride + 4 * q) * (OF ? 4 : 2);
-    char* out_b = static_cast<char*>(c.out) + (ob * c.out_stride + 4 * q) * (OF ? 4 : 2);
-    int stage = 0;
-    for (int step = worker; step < steps; step += workers) {
-      uint4 bn[KB][4];
-      load_b(step + workers, bn);
-      float d[4][4];
-      product(Int<OF && BF ? 3 : 2>(), P == 2 && step >= per_part, d);
-      if (BK != BASE_NONE) wait_but<BS - 1>();
-      const int col = column(step), left = behind(step, col) - 4 * q;
-      const uint32_t at = base_slots + stage * 2048;
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if ((half ? vb : va) && left > 16 * i) {
-            float v[4] = {d[2 * i][2 * half], d[2 * i][2 * half + 1], d[2 * i + 1][2 * half], d[2 * i + 1][2 * half + 1]};
-            if (BK == BASE_F32) {
-              const uint4 w = slot(at + half * 1024 + i * 512);
-              v[0] += __uint_as_float(w.x), v[1] += __uint_as_float(w.y), v[2] += __uint_as_float(w.z), v[3] += __uint_as_float(w.w);
-            } else if (BK == BASE_T) {
-              const uint4 w = slot(at + half * 1024 + i * 512);
-              v[0] += to_float((uint16_t)w.x, T()), v[1] += to_float((uint16_t)(w.x >> 16), T());
-              v[2] += to_float((uint16_t)w.y, T()), v[3] += to_float((uint16_t)(w.y >> 16), T());
-            }
-            char* o = (half ? out_b : out_a) + (int64_t)(col + 16 * i) * (OF ? 4 : 2);
-            if (OF) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-            else *reinterpret_cast<uint2*>(o) = pack4<T>(v);
-          }
-      if (BK != BASE_NONE) fetch_base(base_kind, step + BS * workers, stage);
-      stage = stage + 1 == BS ? 0 : stage + 1;
-      next_b(bn);
-    }
-  };
-  if (kind == 0) columns(Int<BASE_F32>(), Int<0>());
-  else if (kind == 1) columns(Int<BASE_F32>(), Int<1>());
-  else if (kind == 2) columns(Int<BASE_T>(), Int<0>());
-  else if (kind == 3) columns(Int<BASE_NONE>(), Int<0>());
-  else
-    for (int step = worker; step < steps; step += workers) {
-      uint4 bn[KB][4];
-      load_b(step + workers, bn);
-      float d[4][4];
-      product(Int<BF ? 3 : 2>(), P == 2 && step >= per_part, d);
-      const int col = column(step), left = behind(step, col) - 4 * q;
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if ((half ? vb : va) && left > 16 * i) {
-            const float v[4] = {d[2 * i][2 * half], d[2 * i][2 * half + 1], d[2 * i + 1][2 * half], d[2 * i + 1][2 * half + 1]};
-            finish_single(c, half ? ob : oa, col + 4 * q + 16 * i, min(4, left - 16 * i), v);
-          }
-      next_b(bn);
-    }
-}
-
-// ------------------------------------------------------------------------------------ two kernels
-// Every warp has slots of its own in shared memory, filled by asynchronous copies some steps ahead; pointers run along, so that a step
-// is little more than its copies, matrix instructions and stores. Rows behind a tile's last one are computed as copies of its first
-// and not stored.
-
-// h: `share` warps (a power of two) take a tile, each its share of K; a CTA has 8 / share tiles, or with share 8 one of `splits`
-// shares of a tile's K. What its warps have is added in shared memory and goes to the workspace as it is.
-template <int R>
-struct HShape {
-  static constexpr int NT = R / 8, XS = R <= 32 ? 4 : 2;  // steps on the way
-  static constexpr int XB = 16 * 80, XST = XB + NT * 512;   // bytes of a step's x (five pieces of 16 for rows that start anywhere), with A
-  static constexpr int XPART = XS * XST > 16 * R * 4 ? XS * XST : 16 * R * 4, SMEM = 8 * XPART;
-};
-
-template <typename T, int R>
-__global__ void __launch_bounds__(256, R <= 64 ? 2 : 1) adapter_h_kernel(const AdapterCall c) {
-  using S = HShape<R>;
-  constexpr int NT = S::NT, XS = S::XS;
-  extern __shared__ __align__(16) char smem[];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3, share = c.share;
-  const int tile = (int)(blockIdx.x / c.splits) * (8 / share) + warp / share, split = (int)(blockIdx.x % c.splits);
-  const int worker = split * share + warp % share, workers = c.splits * share;
-  const int2* list = reinterpret_cast<const int2*>(c.tiles + 4);
-  int first = 0, matrix = -1, rows = 0;
-  if (tile < c.tiles[0]) {
-    const int2 head = list[tile];
-    first = head.x, matrix = head.y, rows = min(list[tile + 1].x - first, 16);
-  }
-  if (matrix < 0) rows = 0;
-  const int K = (int)c.K, k_steps = matrix < 0 ? 0 : (int)(c.Kp / 32), n = worker < k_steps ? (k_steps - worker - 1) / workers + 1 : 0;
-  const uint32_t slots = (uint32_t)__cvta_generic_to_shared(smem + warp * S::XPART), a_slots = slots + S::XB + lane * 16;
-  const uint16_t* a = c.a + ((int64_t)max(matrix, 0) * k_steps + worker) * (R * 32) + g * 32 + q * 8;
-  const int64_t a_step = (int64_t)workers * (R * 32), x_step = (int64_t)workers * 32;
-  float acc[NT][4];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-  const auto row_of = [&](int r) {
-    const int p = first + (r < rows ? r : 0);
-    return static_cast<const uint16_t*>(c.x) + (int64_t)(c.x_rows ? c.x_rows[p] : p) * c.x_stride;
-  };
-  const auto fetch_a = [&](int stage) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i) copy16(a_slots + stage * S::XST + i * 512, a + i * 256, 16);
-    a += a_step;
-  };
-  const auto multiply = [&](int stage, const uint4& u, const uint4& v) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const uint4 w = slot(a_slots + stage * S::XST + i * 512);
-      mma16(acc[i], u.x, v.x, u.y, v.y, w.x, w.y, T());
-      mma16(acc[i], u.z, v.z, u.w, v.w, w.z, w.w, T());
-    }
-  };
-  if (n == 0) {
-  } else if (c.x_vec) {
-    // a lane's own eight values of its two rows
-    const uint16_t* xa = row_of(g) + worker * 32 + q * 8;
-    const uint16_t* xb = row_of(g + 8) + worker * 32 + q * 8;
-    const uint32_t x_slots = slots + lane * 16;
-    // the last step of all may end inside: zeros from there on
-    const int rest = K - (k_steps - 1) * 32 - q * 8, tail = min(16, max(0, rest * 2));
-    const int tail_at = tail < 16 && (k_steps - 1) % workers == worker ? n - 1 : n;
-    const auto fetch = [&](int i, int stage) {
-      if (i < n) {
-        fetch_a(stage);
-        const int bytes = i == tail_at ? tail : 16;
-        const uint32_t to = x_slots + stage * S::XST;
-        copy16(to, bytes ? xa : static_cast<const uint16_t*>(c.x), bytes);  // a copy of nothing still wants an address
-        copy16(to + 512, bytes ? xb : static_cast<const uint16_t*>(c.x), bytes);
-        xa += x_step, xb += x_step;
-      }
-      commit();
-    };
-#pragma unroll
-    for (int s = 0; s < XS; ++s) fetch(s, s);
-    for (int i = 0; i < n; i += XS) {
-#pragma unroll
-      for (int s = 0; s < XS; ++s) {
-        if (i + s < n) {
-          wait_but<XS - 1>();
-          multiply(s, slot(x_slots + s * S::XST), slot(x_slots + s * S::XST + 512));
-          fetch(i + s + XS, s);
-        }
-      }
-    }
-  } else {
-    // Rows that start anywhere: the aligned pieces of 16 bytes that hold a row's 64 (five), each copied by some lane, and a lane's
-    // eight values shifted out of two of them. What lies in front of a row is not read, nor behind it.
-    const char* piece_at[3];
-    const char *begin[3], *end[3];
-    uint32_t piece_to[3];
-#pragma unroll
-    for (int t = 0; t < 3; ++t) {
-      const int index = min(lane + 32 * t, 79), r = index / 5;
-      begin[t] = reinterpret_cast<const char*>(row_of(r));
-      end[t] = begin[t] + 2 * (int64_t)K;
-      piece_at[t] = begin[t] - (reinterpret_cast<uintptr_t>(begin[t]) & 15) + 16 * (index % 5) + worker * 64;
-      piece_to[t] = slots + index * 16;
-    }
-    const uint32_t ma = (uint32_t)(reinterpret_cast<uintptr_t>(row_of(g)) & 15), mb = (uint32_t)(reinterpret_cast<uintptr_t>(row_of(g + 8)) & 15);
-    const uint32_t from_a = slots + g * 80 + q * 16 + (ma & ~3u), from_b = slots + (g + 8) * 80 + q * 16 + (mb & ~3u);
-    const auto fetch = [&](int i, int stage) {
-      if (i < n) {
-        fetch_a(stage);
-#pragma unroll
-        for (int t = 0; t < 3; ++t) {
-          const uint32_t to = piece_to[t] + stage * S::XST;
-          if (t < 2 || lane < 16) {
-            const int64_t left = end[t] - piece_at[t];
-            if (piece_at[t] >= begin[t]) {
-              const int bytes = (int)(left < 0 ? 0 : left < 16 ? left : 16);
-              copy16(to, bytes ? piece_at[t] : reinterpret_cast<const char*>(c.a), bytes);
-            } else {  // the row's first piece starts in front of it
-              for (int o = 0; o < 16; o += 2) {
-                const char* at = piece_at[t] + o;
-                const uint16_t v = at >= begin[t] && at < end[t] ? *reinterpret_cast<const uint16_t*>(at) : (uint16_t)0;
-                asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + o), "h"(v) : "memory");
-              }
-            }
-          }
-          piece_at[t] += x_step * 2;
-        }
-      }
-      commit();
-    };
-    const auto shifted = [&](uint32_t at, uint32_t m) {
-      uint32_t w[5];
-#pragma unroll
-      for (int i = 0; i < 5; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(at + 4 * i) : "memory");
-      const uint32_t bits = (m & 2) * 8;
-      return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
-                        __funnelshift_r(w[3], w[4], bits));
-    };
-#pragma unroll
-    for (int s = 0; s < XS; ++s) fetch(s, s);
-    for (int i = 0; i < n; i += XS) {
-#pragma unroll
-      for (int s = 0; s < XS; ++s) {
-        if (i + s < n) {
-          wait_but<XS - 1>();
-          __syncwarp();  // the pieces of all lanes
-          const uint4 u = shifted(from_a + s * S::XST, ma), v = shifted(from_b + s * S::XST, mb);
-          multiply(s, u, v);
-          __syncwarp();  // taken by all
-          fetch(i + s + XS, s);
-        }
-      }
-    }
-  }
-  float* mine = reinterpret_cast<float*>(smem + warp * S::XPART);  // over the warp's own slots, which are used up
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    *reinterpret_cast<float2*>(mine + g * R + i * 8 + 2 * q) = make_float2(acc[i][0], acc[i][1]);
-    *reinterpret_cast<float2*>(mine + (g + 8) * R + i * 8 + 2 * q) = make_float2(acc[i][2], acc[i][3]);
-  }
-  if (share > 1) __syncthreads();
-  else __syncwarp();
-  const float* parts = reinterpret_cast<const float*>(smem + (warp - warp % share) * S::XPART);
-  float* to = c.h + ((int64_t)split * c.positions + first) * R;
-  for (int i = (warp % share * 32 + lane) * 4; i < rows * R; i += share * 128) {
-    float4 sum = *reinterpret_cast<const float4*>(parts + i);
-    for (int w = 1; w < share; ++w) {
-      const float4 o = *reinterpret_cast<const float4*>(parts + w * (S::XPART / 4) + i);
-      sum.x += o.x, sum.y += o.y, sum.z += o.z, sum.w += o.w;
-    }
-    *reinterpret_cast<float4*>(to + i) = sum;
-  }
-}
-
-// The columns: `splits` warps take a tile, each every so many steps of 32 columns. The rows' h stays in registers, in pieces.
-template <int RP>
-struct CShape {
-  static constexpr int BB = RP == 16 ? 1024 : RP / 32 * 2048, BST = 2048 + BB;  // bytes of a step: 16 rows of base, B
-  static constexpr int BS = RP == 16 ? 4 : RP == 32 ? 3 : 2, BPART = BS * BST, SMEM = 8 * BPART;
-};
-
-template <typename T, int RP, int P>
-__global__ void __launch_bounds__(256, RP <= 64 ? 2 : 1) adapter_columns_kernel(const AdapterCall c) {
-  using S = CShape<RP>;
-  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
-  constexpr int R = RP * P, KB = RP == 16 ? 1 : RP / 32, BS = S::BS, RF = RP / 16;  // RF: instructions along the rank
-  extern __shared__ __align__(16) char smem[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3, workers = c.splits;
-  const int tile = (int)((blockIdx.x * 8 + warp) / workers), worker = (int)((blockIdx.x * 8 + warp) % workers);
-  if (tile >= c.tiles[0]) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    return;
-  }
-  const int2* list = reinterpret_cast<const int2*>(c.tiles + 4);
-  const int2 head = list[tile];
-  const int first = head.x, matrix = head.y, rows = min(list[tile + 1].x - first, 16);
-  const bool va = g < rows, vb = g + 8 < rows;
-  const int pa = first + (va ? g : 0), pb = first + (vb ? g + 8 : 0);
-  // steps of 32 columns, those of a second part behind those of the first
-  const int Np = (int)c.Np, N = Np * P, per_part = (Np + 31) / 32, steps = per_part * P, n = worker < steps ? (steps - worker - 1) / workers + 1 : 0;
-  const auto column = [&](int step) { return step * 32 + (P == 2 && step >= per_part ? Np - per_part * 32 : 0); };
-  const uint32_t part0 = (uint32_t)__cvta_generic_to_shared(smem + warp * S::BPART), base_slots = part0 + lane * 16;
-  const uint32_t b_slots = part0 + 2048 + lane * (RP == 16 ? 8 : 16);
-  const int64_t oa = c.rows ? c.rows[pa] : pa, ob = c.rows ? c.rows[pb] : pb;
-  const uint16_t* b = c.b + ((int64_t)max(matrix, 0) * N + 4 * (g >> 1) + (g & 1)) * RP + q * (RP == 16 ? 4 : 8);
-  const auto fetch_b = [&](const uint16_t* at, int stage) {
-    if (matrix < 0) return;
-    const uint32_t to = b_slots + stage * S::BST;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint16_t* br = at + (16 * (j >> 1) + 2 * (j & 1)) * RP;
-      if constexpr (RP == 16) {
-        copy8(to + j * 256, br);
-      } else {
-#pragma unroll
-        for (int k = 0; k < KB; ++k) copy16(to + (k * 4 + j) * 512, br + k * 32, 16);
-      }
-    }
-  };
-
-  // the pieces of a part's h, as the instructions take them, and the rows' factors (fp16)
-  uint32_t piece_a[3][RF][2], piece_b[3][RF][2];
-  float fa = 1.f, fb = 1.f;
-  const auto load_h = [&](auto np, int part) {
-    if (matrix < 0) return;
-    constexpr int NP = decltype(np)::value;
-    const float scale = c.scale[matrix / c.per_slot];
-    const int rank = c.ranks[matrix / c.per_slot];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float h[RP / 4];
-#pragma unroll
-      for (int i = 0; i < RP / 4; ++i) h[i] = 0.f;
-      for (int s = 0; s < c.k_splits; ++s) {
-        const float* from = c.h + ((int64_t)s * c.positions + (half ? pb : pa)) * R + part * RP;
-#pragma unroll
-        for (int i = 0; i < RP / 16; ++i) {  // four values of lane q: 4 q of 16 ranks, else 8 q of 32 in two halves
-          const float4 v = *reinterpret_cast<const float4*>(from + (RP == 16 ? 4 * q : (i >> 1) * 32 + 8 * q + 4 * (i & 1)));
-          h[4 * i] += v.x, h[4 * i + 1] += v.y, h[4 * i + 2] += v.z, h[4 * i + 3] += v.w;
-        }
-      }
-      float big = 0.f;
-#pragma unroll
-      for (int i = 0; i < RP / 4; ++i) {
-        const int r = RP == 16 ? 4 * q + i : (i >> 3) * 32 + 8 * q + (i & 7);
-        h[i] = r < rank ? h[i] * scale : 0.f;
-        big = fmaxf(big, fabsf(h[i]));
-      }
-      if (!BF) {  // the four lanes of a row hold all of it (this part's)
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        int ex = 0;
-        if (big > 0.f && isfinite(big)) {
-          (void)frexpf(big, &ex);
-          ex -= 8;  // the largest in [128, 256)
-        }
-#pragma unroll
-        for (int i = 0; i < RP / 4; ++i) h[i] = ldexpf(h[i], -ex);
-        (half ? fb : fa) = ldexpf(1.f, ex);
-      }
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-#pragma unroll
-        for (int i = 0; i < RF; ++i)
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const uint32_t lo = piece(h[4 * i + 2 * w], T()), hi = piece(h[4 * i + 2 * w + 1], T());
-            (half ? piece_b : piece_a)[p][i][w] = lo | (hi << 16);
-          }
-    }
-  };
-  const auto product = [&](auto np, int stage, float (&d)[4][4]) {  // d += h B
-    if (matrix < 0) return;
-    const uint32_t at = b_slots + stage * S::BST;
-#pragma unroll
-    for (int k = 0; k < KB; ++k) {
-      uint4 w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (RP == 16) {
-          asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[j].x), "=r"(w[j].y) : "r"(at + j * 256) : "memory");
-        } else {
-          w[j] = slot(at + (k * 4 + j) * 512);
-        }
-      }
-#pragma unroll
-      for (int i = 2 * k; i < (RP == 16 ? 1 : 2 * k + 2); ++i)
-#pragma unroll
-        for (int p = 0; p < decltype(np)::value; ++p)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma16(d[j], piece_a[p][i][0], piece_b[p][i][0], piece_a[p][i][1], piece_b[p][i][1], i % 2 ? w[j].z : w[j].x, i % 2 ? w[j].w : w[j].y, T());
-    }
-  };
-  const auto zero = [](float (&d)[4][4]) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.f;
-  };
-
-  // Rows of whole fours, parts of whole steps. A lane has four neighbouring columns and the four 16 further on of its two rows.
-  const auto run = [&](auto base_kind, auto out_f32) {
-    constexpr int BK = decltype(base_kind)::value;
-    constexpr bool OF = decltype(out_f32)::value != 0;
-    constexpr int ES = BK == BASE_F32 ? 4 : 2, OS = OF ? 4 : 2;
-    constexpr bool START = BF && !OF;  // the sums start from base: the instructions' own adders are exact enough for 16 bits
-    using NP = Int<BF && OF ? 3 : 2>;
-    const int64_t col0 = worker * 32 + 4 * q;
-    const char* base_a = static_cast<const char*>(c.base) + (oa * c.base_stride + col0) * ES;
-    const char* base_b = static_cast<const char*>(c.base) + (ob * c.base_stride + col0) * ES;
-    char* out_a = static_cast<char*>(c.out) + (oa * c.out_stride + col0) * OS;
-    char* out_b = static_cast<char*>(c.out) + (ob * c.out_stride + col0) * OS;
-    const uint16_t* b_at = b + (int64_t)worker * 32 * RP;
-    const int64_t stride = (int64_t)workers * 32;
-    // the last step of all may end inside
-    const int rest = N - (steps - 1) * 32 - 4 * q, last = rest <= 16 && (steps - 1) % workers == worker ? n - 1 : n;
-    const auto fetch = [&](int i, int stage) {
-      if (i < n) {
-        fetch_b(b_at, stage);
-        b_at += stride * RP;
-        if (BK != BASE_NONE) {
-          const bool in0 = i != last || rest > 0, in1 = i != last;
-          const uint32_t to = base_slots + stage * S::BST;
-          if constexpr (ES == 4) {
-            if (in0) copy16(to, base_a, 16), copy16(to + 1024, base_b, 16);
-            if (in1) copy16(to + 512, base_a + 16 * ES, 16), copy16(to + 1536, base_b + 16 * ES, 16);
-          } else {
-            if (in0) copy8(to, base_a), copy8(to + 1024, base_b);
-            if (in1) copy8(to + 512, base_a + 16 * ES), copy8(to + 1536, base_b + 16 * ES);
-          }
-          base_a += stride * ES, base_b += stride * ES;
-        }
-      }
-      commit();
-    };
-    const auto take_base = [&](int stage, int i, int half, float (&v)[4]) {
-      const uint4 w = slot(base_slots + stage * S::BST + half * 1024 + i * 512);
-      if (BK == BASE_F32) {
-        v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y), v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
-      } else {
-        v[0] = to_float((uint16_t)w.x, T()), v[1] = to_float((uint16_t)(w.x >> 16), T());
-        v[2] = to_float((uint16_t)w.y, T()), v[3] = to_float((uint16_t)(w.y >> 16), T());
-      }
-    };
-#pragma unroll
-    for (int s = 0; s < BS; ++s) fetch(s, s);
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // h is there
-    int part = P == 2 && worker >= per_part;
-    load_h(NP(), part);
-    for (int i0 = 0; i0 < n; i0 += BS) {
-#pragma unroll
-      for (int s = 0; s < BS; ++s) {
-        const int i = i0 + s;
-        if (i < n) {
-          if (P == 2 && part == 0 && worker + i * workers >= per_part) part = 1, load_h(NP(), part);
-          wait_but<BS - 1>();
-          float d[4][4];
-          if (START && BK != BASE_NONE) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                float v[4];
-                take_base(s, u, half, v);
-                d[2 * u][2 * half] = v[0], d[2 * u][2 * half + 1] = v[1], d[2 * u + 1][2 * half] = v[2], d[2 * u + 1][2 * half + 1] = v[3];
-              }
-          } else {
-            zero(d);
-          }
-          product(NP(), s, d);
-          const bool in0 = i != last || rest > 0, in1 = i != last;
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              float v[4] = {d[2 * u][2 * half], d[2 * u][2 * half + 1], d[2 * u + 1][2 * half], d[2 * u + 1][2 * half + 1]};
-              if (!BF) {
-                const float f = half ? fb : fa;
-                v[0] *= f, v[1] *= f, v[2] *= f, v[3] *= f;
-              }
-              if (!START && BK != BASE_NONE) {
-                float w[4];
-                take_base(s, u, half, w);
-                v[0] += w[0], v[1] += w[1], v[2] += w[2], v[3] += w[3];
-              }
-              if ((half ? vb : va) && (u ? in1 : in0)) {
-                char* o = (half ? out_b : out_a) + 16 * u * OS;
-                if (OF) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-                else *reinterpret_cast<uint2*>(o) = pack4<T>(v);
-              }
-            }
-          out_a += stride * OS, out_b += stride * OS;
-          fetch(i + BS, s);
-        }
-      }
-    }
-  };
-  if (c.kind == 0) return run(Int<BASE_F32>(), Int<0>());
-  if (c.kind == 1) return run(Int<BASE_F32>(), Int<1>());
-  if (c.kind == 2) return run(Int<BASE_T>(), Int<0>());
-  if (c.kind == 3) return run(Int<BASE_NONE>(), Int<0>());
-  // Any types and alignment: the sums go through shared memory, so that a warp reads and writes 32 neighbouring columns of a row at
-  // a time; base is read a step ahead.
-  using NP = Int<BF ? 3 : 2>;
-  float next[16];
-  const auto base_of = [&](int step) {
-    const int64_t col = column(step) + lane;
-    const bool in = step < steps && col < (P == 2 && step < per_part ? Np : N);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int64_t row = __shfl_sync(0xffffffffu, r < 8 ? oa : ob, (r & 7) * 4);
-      next[r] = in && c.base && r < rows ? element(c.base, row * c.base_stride + col, c.base_dtype) : 0.f;
-    }
-  };
-#pragma unroll
-  for (int s = 0; s < BS; ++s) {
-    const int step = worker + s * workers;
-    if (step < steps) fetch_b(b + (int64_t)column(step) * RP, s);
-    commit();
-  }
-  base_of(worker);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  int part = P == 2 && worker >= per_part, stage = 0;
-  load_h(NP(), part);
-  for (int step = worker; step < steps; step += workers) {
-    if (P == 2 && part == 0 && step >= per_part) part = 1, load_h(NP(), part);
-    wait_but<BS - 1>();
-    float d[4][4], mine[16];
-    zero(d);
-    product(NP(), stage, d);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) mine[r] = next[r];
-    base_of(step + workers);
-    const uint32_t at = part0 + stage * S::BST;
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float f = half ? fb : fa;
-        asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(at + (g + 8 * half) * 128 + (16 * u + 4 * q) * 4), "f"(d[2 * u][2 * half] * f),
-                     "f"(d[2 * u][2 * half + 1] * f), "f"(d[2 * u + 1][2 * half] * f), "f"(d[2 * u + 1][2 * half + 1] * f)
-                     : "memory");
-      }
-    __syncwarp();
-    const int64_t col = column(step) + lane;
-    const bool in = col < (P == 2 && step < per_part ? Np : N);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int64_t row = __shfl_sync(0xffffffffu, r < 8 ? oa : ob, (r & 7) * 4);
-      float v;
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at + r * 128 + lane * 4) : "memory");
-      v += mine[r];
-      if (in && r < rows) {
-        const int64_t o = row * c.out_stride + col;
-        if (c.out_dtype == DST_OUT_F32) static_cast<float*>(c.out)[o] = v;
-        else if (c.out_dtype == DST_OUT_BF16) static_cast<__nv_bfloat16*>(c.out)[o] = __float2bfloat16_rn(v);
-        else static_cast<__half*>(c.out)[o] = __float2half_rn(v);
-      }
-    }
-    __syncwarp();
-    if (step + BS * workers < steps) fetch_b(b + (int64_t)column(step + BS * workers) * RP, stage);
-    commit();
-    stage = stage + 1 == BS ? 0 : stage + 1;
-  }
-}
-
-template <typename T, int RP, int P>
-int launch_cluster(const AdapterCall& c, int64_t max_tiles, cudaStream_t st) {
-  using S = Shape<T, RP, P>;
-  auto kernel = adapter_kernel<T, RP, P>;
-  if (S::SMEM > 48 * 1024) DST_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(max_tiles * c.ctas)), cfg.blockDim = dim3(WARPS * 32), cfg.dynamicSmemBytes = S::SMEM, cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = c.ctas, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr, cfg.numAttrs = 1;
-  DST_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, c));
-  return DST_OK;
-}
-
-template <typename T, int RP, int P>
-int launch(AdapterCall c, int64_t max_tiles, cudaStream_t st) {
-  if (c.ctas) return launch_cluster<T, RP, P>(c, max_tiles, st);
-  using H = HShape<RP * P>;
-  using C = CShape<RP>;
-  auto h_kernel = adapter_h_kernel<T, RP * P>;
-  auto c_kernel = adapter_columns_kernel<T, RP, P>;
-  DST_CUDA_TRY(cudaFuncSetAttribute(h_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, H::SMEM));
-  DST_CUDA_TRY(cudaFuncSetAttribute(c_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-  const int columns = c.splits;
-  c.splits = c.k_splits;
-  h_kernel<<<(unsigned)(cdiv64(max_tiles * c.share, 8) * c.k_splits), 256, H::SMEM, st>>>(c);
-  DST_CUDA_TRY(cudaGetLastError());
-  c.splits = columns;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)cdiv64(max_tiles * columns, 8)), cfg.blockDim = dim3(256), cfg.dynamicSmemBytes = C::SMEM, cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr, cfg.numAttrs = 1;
-  DST_CUDA_TRY(cudaLaunchKernelEx(&cfg, c_kernel, c));
-  return DST_OK;
-}
-
-template <typename T>
-int launch_for(const AdapterCall& c, int rank_padded, int64_t max_tiles, cudaStream_t st) {
-  if (c.parts == 1) {
-    if (rank_padded == 16) return launch<T, 16, 1>(c, max_tiles, st);
-    if (rank_padded == 32) return launch<T, 32, 1>(c, max_tiles, st);
-    if (rank_padded == 64) return launch<T, 64, 1>(c, max_tiles, st);
-    if (rank_padded == 128) return launch<T, 128, 1>(c, max_tiles, st);
-  } else if (c.parts == 2) {
-    if (rank_padded == 16) return launch<T, 16, 2>(c, max_tiles, st);
-    if (rank_padded == 32) return launch<T, 32, 2>(c, max_tiles, st);
-    if (rank_padded == 64) return launch<T, 64, 2>(c, max_tiles, st);
-  }
-  return DST_ERR_UNSUPPORTED;
-}
-
-// How a call is cut: CTAs of a cluster (0: two kernels); warps of a tile for h inside a CTA and CTAs of a tile; warps of a tile for
-// the columns
+// How a call is cut: CTAs of a cluster (0: two kernels); warps of 16 rows for h inside a CTA and CTAs of them; those for the columns;
+// whether the row blocks of a tile share A and B (`shares`: they may, by types and alignment)
 struct Cut {
-  int ctas, share, k_splits, columns;
+  int ctas, share, k_splits, columns, shared;
 };
-int env(const char* n, int d) { return getenv(n) ? atoi(getenv(n)) : d; }
-Cut cut_of(int64_t max_tiles, int64_t K_padded, int64_t N) {
-  const int64_t sms = sm_count();
-  Cut cut{0, 8, 1, 1};
-  if (max_tiles <= env("DST_FEW", 32)) {
+Cut cut_of(int64_t max_tiles, int tile, int64_t K_padded, int64_t N, int rank_padded, bool shares) {
+  const int64_t sms = sm_count(), blocks = max_tiles * (tile / 16);
+  Cut cut{0, 8, 1, 1, 0};
+  // Up to 48 blocks the cluster's one launch costs the host 5 us less (11 against 16 a call) and the device as much: 1 row of 4096 x
+  // 4096 4.2 us against 4.1, 333 rows 8.0 against 8.2, 48 pairs (rank 16 twice) 13.1 against 14.4 with their plan; 64 rows of 37 adapters (53 blocks) through 11008 x 4096 14.9 against 11.2
+  if (blocks <= 48) {
     cut.ctas = 1;
-    while (cut.ctas < MAX_CTAS && max_tiles * cut.ctas * 2 <= 2 * sms) cut.ctas *= 2;
+    while (cut.ctas < ADAPTER_MAX_CTAS && max_tiles * cut.ctas * 2 <= 2 * sms) cut.ctas *= 2;
     return cut;
   }
-  const int64_t want_h = env("DST_WH", 32) * sms, want_c = env("DST_WC", 32) * sms;
-  const auto warps = [&](int64_t steps, int64_t want, int64_t least) {  // of a tile: a power of two, `least` steps a warp or more
+  const auto warps = [&](int64_t steps, int64_t want, int64_t least) {  // of a block: a power of two, `least` steps a warp or more
     int64_t n = 1;
-    while (max_tiles * n < want && n * 2 * least <= steps) n *= 2;
+    while (blocks * n < want && n * 2 * least <= steps) n *= 2;
     return (int)n;
   };
-  const int h = warps(K_padded / 32, want_h, env("DST_LH", 4));
-  cut.share = std::min(h, 8), cut.k_splits = std::min(std::max(h / 8, 1), 16);
-  cut.columns = warps(N / 32, want_c, env("DST_LC", 4));
+  // Warps enough for some waves, with steps enough for each to pay for its start. Measured, us: 64 rows as above with at least 2 / 4 / 8 /
+  // 16 steps 13.8 / 11.2 / 14.7 / 19.7, 4000 rows of rank 64 47 / 44 / 41 / 43; 2048 tokens' pairs through 64 experts with 8 / 16 / 32 / 64
+  // warps an SM for the columns 82 / 77 / 70 / 70, 4000 rows of rank 64 that share B 43 / 37 / 39 / -
+  cut.shared = tile == 128 && rank_padded >= 64 && shares;
+  const int least = blocks <= sms ? 4 : 8;
+  const int h = warps(K_padded / 64, 8 * sms, least);
+  cut.columns = warps(N / 32, (cut.shared ? 16 : 32) * sms, least);
+  cut.share = cut.shared ? 1 : std::min(h, 8), cut.k_splits = std::min(cut.shared ? h : std::max(h / 8, 1), 16);
   return cut;
 }
 
 }  // namespace
 }  // namespace dst
 
+// Tiles of 128 rows let eight warps share A and B where the rank is 64 or more, once requests fill them (lower ranks take their
+// row blocks apart). Rank 64: 4000 rows, float32 results 37 us against 41 in tiles of 16, 1654 rows 30 against 21.
+extern "C" int dst_adapter_tile(int64_t rows, int64_t bins) { return rows >= 20 * (int64_t)dst::sm_count() && rows >= 128 * bins ? 128 : 16; }
+
 extern "C" size_t dst_adapter_workspace_bytes(const dst_adapters* w, const dst_adapter_rows* plan) {
   using namespace dst;
   if (!w || !plan || plan->max_tiles <= 0 || plan->positions <= 0 || w->parts < 1 || w->rank_padded < 1 || w->K_padded < 1 || w->N < 1)
     return 0;
-  const Cut cut = cut_of(plan->max_tiles, w->K_padded, w->N);
-  return cut.ctas ? 0 : (size_t)cut.k_splits * plan->positions * w->parts * w->rank_padded * sizeof(float);
+  // for either form of the rows: which one it is depends on the tensors' alignment too
+  const Cut one = cut_of(plan->max_tiles, plan->tile, w->K_padded, w->N, w->rank_padded, true);
+  const Cut two = cut_of(plan->max_tiles, plan->tile, w->K_padded, w->N, w->rank_padded, false);
+  return one.ctas ? 0 : (size_t)std::max(one.k_splits, two.k_splits) * plan->positions * w->parts * w->rank_padded * sizeof(float);
 }
 
 extern "C" int dst_adapter_apply(const dst_adapters* w, const dst_adapter_rows* plan, const void* x, int64_t x_stride, const void* base,
@@ -1019,8 +62,8 @@ extern "C" int dst_adapter_apply(const dst_adapters* w, const dst_adapter_rows* 
       (w->dtype != DST_ACT_BF16 && w->dtype != DST_ACT_F16) || w->K <= 0 || w->N <= 0 ||
       w->matrices_per_slot <= 0 || plan->max_tiles < 0)
     return DST_ERR_BAD_ARG;
-  if (w->parts < 1 || w->N % w->parts != 0 || w->K_padded < w->K || w->K_padded % 32 != 0 || x_stride < w->K || out_stride < w->N ||
-      (base && base_stride < w->N) || plan->max_tiles > 0x00ffffff || plan->positions < 0 || w->N > (1 << 24) || w->K_padded > (1 << 24) || plan->tile != DST_ADAPTER_TILE)
+  if (w->parts < 1 || w->N % w->parts != 0 || w->K_padded < w->K || w->K_padded % 64 != 0 || x_stride < w->K || out_stride < w->N ||
+      (base && base_stride < w->N) || plan->max_tiles > 0x00ffffff || plan->positions < 0 || w->N > (1 << 24) || w->K_padded > (1 << 24) || (plan->tile != 16 && plan->tile != 128))
     return DST_ERR_BAD_SHAPE;
   if (plan->max_tiles == 0) return DST_OK;
   if (!w->a || !w->b || !w->scale || !w->ranks || !plan->tiles || !x || !out) return DST_ERR_BAD_ARG;
@@ -1031,22 +74,22 @@ extern "C" int dst_adapter_apply(const dst_adapters* w, const dst_adapter_rows* 
   c.a = static_cast<const uint16_t*>(w->a), c.b = static_cast<const uint16_t*>(w->b), c.scale = w->scale, c.ranks = w->ranks;
   c.per_slot = w->matrices_per_slot, c.K = w->K, c.Kp = w->K_padded, c.Np = w->N / w->parts, c.parts = w->parts;
   c.base = base, c.base_dtype = base_dtype, c.base_stride = base_stride, c.out = out, c.out_dtype = out_dtype, c.out_stride = out_stride;
-  const auto aligned = [](const void* p, int64_t stride, int n, int size) { return reinterpret_cast<uintptr_t>(p) % (n * size) == 0 && stride % n == 0; };
-  c.x_vec = aligned(x, x_stride, 8, 2);
-  const int own = w->dtype == DST_ACT_BF16 ? DST_OUT_BF16 : DST_OUT_F16;
+  const auto aligned = [](const void* p, int64_t stride, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0; };
+  c.x_vec = aligned(x, x_stride, 2);
+  const int own = w->dtype == DST_ACT_BF16 ? DST_OUT_BF16 : DST_OUT_F16, out_size = out_dtype == DST_OUT_F32 ? 4 : 2;
   c.kind = -1;
-  if (c.Np % (w->parts == 1 ? 4 : 32) == 0 && aligned(out, out_stride, 4, out_dtype == DST_OUT_F32 ? 4 : 2) &&
-      (!base || aligned(base, base_stride, 4, base_dtype == DST_OUT_F32 ? 4 : 2))) {
+  if (c.Np % (w->parts == 1 ? 16 / out_size : 32) == 0 && aligned(out, out_stride, out_size) &&
+      (!base || aligned(base, base_stride, base_dtype == DST_OUT_F32 ? 4 : 2))) {
     if (base && base_dtype == DST_OUT_F32 && (out_dtype == own || out_dtype == DST_OUT_F32)) c.kind = out_dtype == own ? 0 : 1;
     else if (out_dtype == own && (!base || base_dtype == own)) c.kind = base ? 2 : 3;
   }
-  const Cut cut = cut_of(plan->max_tiles, w->K_padded, w->N);
-  c.ctas = cut.ctas, c.share = cut.share, c.k_splits = cut.k_splits, c.splits = cut.columns, c.positions = plan->positions, c.h = static_cast<float*>(workspace);
+  const Cut cut = cut_of(plan->max_tiles, plan->tile, w->K_padded, w->N, w->rank_padded, c.x_vec && c.kind >= 0);
+  c.sub = plan->tile / 16, c.shared = cut.shared, c.ctas = cut.ctas, c.share = cut.share, c.k_splits = cut.k_splits, c.splits = cut.columns, c.positions = plan->positions, c.h = static_cast<float*>(workspace);
   if (!cut.ctas) {
     if (!workspace || workspace_bytes < dst_adapter_workspace_bytes(w, plan)) return DST_ERR_BAD_ARG;
     if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return DST_ERR_ALIGNMENT;
   }
   auto st = static_cast<cudaStream_t>(stream);
-  return w->dtype == DST_ACT_BF16 ? launch_for<__nv_bfloat16>(c, w->rank_padded, plan->max_tiles, st)
-                                  : launch_for<__half>(c, w->rank_padded, plan->max_tiles, st);
+  return w->dtype == DST_ACT_BF16 ? adapter_launch_bf16(c, w->rank_padded, plan->max_tiles, st)
+                                  : adapter_launch_f16(c, w->rank_padded, plan->max_tiles, st);
 }

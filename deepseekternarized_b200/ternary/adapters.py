@@ -21,7 +21,6 @@ from ..kernels import ternary_b200 as kb
 
 _UNAVAILABLE = "the B200 adapters are unavailable: {} not on a CUDA device and this backend has no CPU path"
 _PADDED_RANKS = (16, 32, 64, 128)
-_TILE = _lib.ADAPTER_TILE
 
 
 def _int32(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -36,21 +35,23 @@ def _int32(t: torch.Tensor, what: str) -> torch.Tensor:
 
 @lru_cache(4096)
 def _plan_sizes(n_rows: int, n_adapters: int):
-    """(most tiles, first int32 of order / bins / offsets in the plan's buffer, workspace bytes) of a plan's sizes."""
+    """(tile height, most tiles, first int32 of order / bins / offsets in the plan's buffer, workspace bytes) of a plan's sizes."""
     if n_adapters < 1 or n_adapters > 4095 or n_rows < 0:
         raise RuntimeError("a plan takes 1 to 4095 adapters")
     lib = kb._require("auto")
-    at = int(lib.dst_adapter_tile_capacity(n_rows, n_adapters + 1, _TILE))
-    return min(n_rows, -(-n_rows // _TILE) + n_adapters + 1), at, at + n_rows, at + 2 * n_rows, int(lib.dst_adapter_plan_workspace_bytes(n_rows, n_adapters))
+    tile = int(lib.dst_adapter_tile(n_rows, n_adapters + 1))
+    at = int(lib.dst_adapter_tile_capacity(n_rows, n_adapters + 1, tile))
+    return tile, min(n_rows, -(-n_rows // tile) + n_adapters + 1), at, at + n_rows, at + 2 * n_rows, int(lib.dst_adapter_plan_workspace_bytes(n_rows, n_adapters))
 
 
 @lru_cache(4096)
 def _pair_sizes(pairs: int, n_adapters: int, n_experts: int):
-    """(most tiles, int64 words of the tile list, of all, workspace bytes) of an expert plan's sizes."""
+    """(tile height, most tiles, int64 words of the tile list, of all, workspace bytes) of an expert plan's sizes."""
     lib = kb._require("auto")
     bins = (n_adapters + 1) * n_experts
-    tiles = -(-int(lib.dst_adapter_tile_capacity(pairs, bins, _TILE)) // 2)
-    return min(pairs, -(-pairs // _TILE) + bins), tiles, pairs + n_experts + 1 + tiles + -(-pairs // 2), \
+    tile = int(lib.dst_adapter_tile(pairs, bins))
+    tiles = -(-int(lib.dst_adapter_tile_capacity(pairs, bins, tile)) // 2)
+    return tile, min(pairs, -(-pairs // tile) + bins), tiles, pairs + n_experts + 1 + tiles + -(-pairs // 2), \
         int(lib.dst_adapter_plan_experts_workspace_bytes(pairs, n_experts))
 
 
@@ -85,15 +86,15 @@ class AdapterPlan:
             if offsets.device != dev:
                 raise RuntimeError("offsets and slots must share one device")
             p_offsets = offsets.data_ptr()
-        max_tiles, at_order, at_bins, at_offsets, ws_bytes = _plan_sizes(n_rows, n_adapters)
-        self.n_rows, self.n_adapters, self.max_tiles, self.device = n_rows, n_adapters, max_tiles, dev
+        tile, max_tiles, at_order, at_bins, at_offsets, ws_bytes = _plan_sizes(n_rows, n_adapters)
+        self.n_rows, self.n_adapters, self.tile, self.max_tiles, self.device = n_rows, n_adapters, tile, max_tiles, dev
         # one buffer: tiles, order, bins, offsets
         self._buf = torch.empty(at_offsets + n_adapters + 2, dtype=torch.int32, device=dev)
         self._at = at_order, at_bins, at_offsets
         base = self._buf.data_ptr()
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         with kb._guard(dev):
-            _lib.check(lib.dst_adapter_plan(p_offsets, slots.data_ptr(), slots.size(0), n_rows, n_adapters, _TILE, base + 4 * at_order,
+            _lib.check(lib.dst_adapter_plan(p_offsets, slots.data_ptr(), slots.size(0), n_rows, n_adapters, tile, base + 4 * at_order,
                                             base + 4 * at_bins, base + 4 * at_offsets, base, ws.data_ptr() if ws is not None else None, ws_bytes,
                                             kb._stream(slots)))
         self._c = None
@@ -102,7 +103,7 @@ class AdapterPlan:
         """The C struct of these rows, made when a projection asks for it first."""
         if self._c is None:
             base = self._buf.data_ptr()
-            self._c = ctypes.byref(_lib.AdapterRowsC(base + 4 * self._at[0], base + 4 * self._at[0], base, self.max_tiles, self.n_rows, _TILE))
+            self._c = ctypes.byref(_lib.AdapterRowsC(base + 4 * self._at[0], base + 4 * self._at[0], base, self.max_tiles, self.n_rows, self.tile))
         return self._c
 
     @property
@@ -133,7 +134,7 @@ class ExpertPlan:
         T, k = ids.shape
         P, n, dev = T * k, plan.n_adapters, plan.device
         self.tokens, self.n_rows, self.n_adapters, self.n_experts, self.device = T, P, n, n_experts, dev
-        self.max_tiles, tiles, words, ws_bytes = _pair_sizes(P, n, n_experts)
+        self.tile, self.max_tiles, tiles, words, ws_bytes = _pair_sizes(P, n, n_experts)
         # one buffer of 64-bit words: order, offsets, tiles, x rows
         self._buf = torch.empty(words, dtype=torch.int64, device=dev)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
@@ -142,7 +143,7 @@ class ExpertPlan:
         self._tiles = p_offsets + 8 * (n_experts + 1)
         self._x_rows = self._tiles + 8 * tiles
         with kb._guard(dev):
-            _lib.check(lib.dst_adapter_plan_experts(ids.data_ptr(), T, k, n_experts, src + 4 * plan._at[0], src + 4 * plan._at[1], n, _TILE,
+            _lib.check(lib.dst_adapter_plan_experts(ids.data_ptr(), T, k, n_experts, src + 4 * plan._at[0], src + 4 * plan._at[1], n, self.tile,
                                                     base, p_offsets, self._x_rows, self._tiles, ws.data_ptr() if ws is not None else None,
                                                     ws_bytes, kb._stream(ids)))
         self._order = self._offsets = None
@@ -152,7 +153,7 @@ class ExpertPlan:
         """The C struct of the pairs with x rows of the tokens or of the pairs, made when a projection asks for it first."""
         c = self._c[pair_rows]
         if c is None:
-            c = self._c[pair_rows] = ctypes.byref(_lib.AdapterRowsC(None, None if pair_rows else self._x_rows, self._tiles, self.max_tiles, self.n_rows, _TILE))
+            c = self._c[pair_rows] = ctypes.byref(_lib.AdapterRowsC(None, None if pair_rows else self._x_rows, self._tiles, self.max_tiles, self.n_rows, self.tile))
         return c
 
     @property
@@ -188,7 +189,7 @@ class LowRankAdapters:
         if torch.device(device).type != "cuda":
             raise RuntimeError(_UNAVAILABLE.format("the adapters are"))
         self.n_adapters, self.K, self.N, self.rank, self.dtype, self.experts, self.parts = n_adapters, K, N, rank, dtype, experts, parts
-        E, Kp = experts or 1, -(-K // 32) * 32
+        E, Kp = experts or 1, -(-K // 64) * 64
         # A in steps of 32 values of K, the ranks of a step together: what a warp reads at once is one stretch of memory
         self._a = torch.zeros(n_adapters, E, Kp // 32, parts, self.rank_padded, 32, dtype=dtype, device=device)
         rows = n_adapters * E * N  # and 31 more, which the last step of columns may read
@@ -274,7 +275,7 @@ class LowRankAdapters:
             raise RuntimeError("adapters, plan and tensors must share one device")
         if P:
             c = plan._rows_c(pair_rows)
-            sizes = plan.max_tiles, P
+            sizes = plan.max_tiles, P, plan.tile
             ws_bytes = self._ws_bytes.get(sizes)
             if ws_bytes is None:  # by sizes alone
                 ws_bytes = self._ws_bytes[sizes] = int(kb._require("auto").dst_adapter_workspace_bytes(self._ref, c))

@@ -300,7 +300,7 @@ int dst_moe_layer(const void* x_bf16, const float* weights, const int32_t* ids, 
  * and the combine take as order and offsets. x_rows [T * top_k] = the position's token. tiles
  * [dst_adapter_tile_capacity(T * top_k, (n + 1) * E, tile)]: matrix adapter * E + expert. E <= 4096.
  */
-enum { DST_ADAPTER_TILE = 16 }; /* the rows of a tile that dst_adapter_apply takes */
+int dst_adapter_tile(int64_t rows, int64_t bins); /* the tile height that suits a plan of so many rows and bins: 16 or 128 */
 int64_t dst_adapter_tile_capacity(int64_t rows, int64_t bins, int tile);
 size_t dst_adapter_plan_workspace_bytes(int64_t rows, int64_t n);
 int dst_adapter_plan(const int32_t* offsets, const int32_t* slots, int64_t requests, int64_t rows, int64_t n, int tile, int32_t* order,
@@ -317,7 +317,7 @@ int dst_adapter_plan_experts(const int32_t* ids, int64_t T, int top_k, int64_t E
  * x); 31 more rows behind the last matrix of B can be read. Part p of the columns (N / parts each) takes rows p * rank_padded ..
  * of A. matrices_per_slot: matrices of one adapter (experts; 1 beside a dense projection), adapter a = m / matrices_per_slot with
  * the rank ranks[a] <= rank_padded; what lies behind it is finite and counts for nothing (rank 0: the base alone).
- * rank_padded 16, 32, 64 or 128; parts 1 or 2 with parts * rank_padded <= 128; K_padded a multiple of 32.
+ * rank_padded 16, 32, 64 or 128; parts 1 or 2 with parts * rank_padded <= 128; K_padded a multiple of 64.
  * rows / x_rows: base / out row and x row of a position (NULL: the position). base (DST_OUT_* type) may be NULL (zeros) or the
  * same rows as out; x may not overlap out. Strides in elements. positions: rows of the plan (pairs of a layer). Workspace (16-byte
  * aligned): dst_adapter_workspace_bytes, by sizes and rank_padded, parts, tile alone; 0 for few tiles.

@@ -201,7 +201,7 @@ def check_plan(plan, slots, n):
     tiles = tile_list(plan)
     assert tiles[-1, 0] == len(b) and (len(b) == 0 or tiles[0, 0] == 0)
     for (a, m), (e, _) in zip(tiles[:-1], tiles[1:]):
-        assert 0 < e - a <= _lib.ADAPTER_TILE and set(b[order[a:e]].tolist()) == {n if m < 0 else int(m)}
+        assert 0 < e - a <= plan.tile and set(b[order[a:e]].tolist()) == {n if m < 0 else int(m)}
 
 
 @gpu
@@ -253,7 +253,7 @@ def test_plan_of_experts(T, k, E, n):
         assert tiles[-1, 0] == len(order) and (len(order) == 0 or tiles[0, 0] == 0)
         for (a, m), (e, _) in zip(tiles[:-1], tiles[1:]):
             pairs = order[a:e]
-            assert 0 < e - a <= _lib.ADAPTER_TILE and {(int(b[i]), int(flat[i])) for i in pairs} == ({(m // E, m % E)} if m >= 0 else {(n, int(flat[pairs[0]]))})
+            assert 0 < e - a <= p.tile and {(int(b[i]), int(flat[i])) for i in pairs} == ({(m // E, m % E)} if m >= 0 else {(n, int(flat[pairs[0]]))})
 
 
 def test_plans_and_adapters_refuse_without_a_gpu_or_with_bad_arguments():
@@ -319,7 +319,7 @@ def test_abi_argument_checks():
 
     assert apply(plan=dict(max_tiles=0)) == _lib.OK
     for kw, want in ((dict(w=dict(a=None)), 1), (dict(w=dict(ranks=None)), 1), (dict(w=dict(dtype=2)), 1), (dict(w=dict(K=0)), 1), (dict(bt=3), 1), (dict(ot=-1), 1),
-                     (dict(x=None), 1), (dict(out=None), 1), (dict(w=dict(parts=3)), 2), (dict(w=dict(K_padded=32)), 2), (dict(w=dict(K_padded=72)), 2),
+                     (dict(x=None), 1), (dict(out=None), 1), (dict(w=dict(parts=3)), 2), (dict(w=dict(K_padded=32)), 2), (dict(w=dict(K_padded=96)), 2),
                      (dict(xs=63), 2), (dict(bs=63), 2), (dict(os_=63), 2), (dict(w=dict(a=p + 2)), 5), (dict(plan=dict(max_tiles=400, positions=6400), ws=None), 1),
                      (dict(plan=dict(max_tiles=400, positions=6400), wsb=6400), 1), (dict(plan=dict(max_tiles=400, positions=6400), ws=p + 8), 5),
                      (dict(plan=dict(tile=48)), 2), (dict(plan=dict(tiles=p + 4)), 5),
