@@ -19,7 +19,7 @@ SOURCES = ["api.cu", "format_kernels.cu", "layout_kernels.cu", "gemm_generic.cu"
            "moe_kernels.cu", "moe_layer.cu", "route_group.cu", "adapter_plan.cu", "adapter_gemm.cu",
            "adapter_gemm_bf16.cu", "adapter_gemm_f16.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-shared",
-              "-Xcompiler", "-fPIC"]
+              "-Xcompiler", "-fPIC", "--threads", "0"]  # sources side by side
 
 OK, ERR_BAD_ARG, ERR_BAD_SHAPE, ERR_BAD_OFFSETS, ERR_UNSUPPORTED, ERR_ALIGNMENT, ERR_CUDA, ERR_TIMEOUT, ERR_TOO_LARGE = range(9)
 NOALLOC_SCRATCH_BYTES = 8 * 1024 * 1024 + 16384

@@ -23,9 +23,9 @@ namespace cg = cooperative_groups;
 
 constexpr int THREADS = 1024, WARPS = 32, SMALL = 1024, MAX_CTAS = 8;
 constexpr int64_t CLUSTER_ENTRIES = 131072;  // entries and bins of the cluster's form
-constexpr int CLUSTER_BINS = 1024;
-constexpr int64_t RANK_ROWS = 192, RANK_PAIRS = 384;  // beyond, a cluster is faster: 128 / 256 / 1024 rows 4.6 / 5.9 / 27 us against 5.8 / 5.8 / 6.3,
-                                                        // 256 / 512 pairs (with their adapters) 10.0 / 14.3 against 13.1 / 14.3
+constexpr int CLUSTER_BINS = 2048;
+constexpr int64_t RANK_ROWS = 192, RANK_PAIRS = 256;  // beyond, a cluster is faster: 128 / 256 / 1024 rows 4.6 / 5.9 / 27 us against 5.8 / 5.8 / 6.3,
+                                                        // 64 / 512 pairs 3.4 / 10 against 6.8 / 6.8
 
 // The bin of a row: the request that it lies in is the last one that starts at or before it.
 __device__ __forceinline__ int bin_of_row(const int32_t* __restrict__ offsets, const int32_t* __restrict__ slots, int64_t requests, int64_t row,
@@ -152,18 +152,21 @@ __global__ void __launch_bounds__(THREADS) small_kernel(const Plan a) {
 }
 
 // ------------------------------------------------------------------------------------ one cluster
-// A warp counts and places a run of consecutive entries of its own. Rows: keys are bins. Pairs: taken in the order of the tokens'
-// plan, which is the bins', and sorted by expert; a tile starts where expert or bin change and at multiples of its height.
-template <bool PAIRS>
+// A warp counts and places a run of consecutive entries of its own. ROWS: keys are bins. PAIRS: keys are expert and bin, where the
+// counters hold as many. BY_ORDER: pairs are taken in the order of the tokens' plan, which is the bins', and sorted by expert; a tile
+// starts where expert or bin change and at multiples of its height.
+enum { ROWS, PAIRS, BY_ORDER };
+
+template <int MODE>
 __global__ void __launch_bounds__(THREADS) cluster_kernel(const Plan a) {
   extern __shared__ int32_t sh[];
   const cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
-  const int nb = PAIRS ? a.E : a.n + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n1 = a.n + 1, nb = MODE == BY_ORDER ? a.E : MODE == PAIRS ? a.E * n1 : n1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int32_t* totals = sh;                   // [nb] this block's, read by the others
   int32_t* start = totals + nb;           // [nb] of this block's entries
   int32_t* global = start + nb;           // [nb + 1] of all
-  int32_t* tstart = global + nb + 1;      // [nb + 1] rows: first tile of a bin
+  int32_t* tstart = global + nb + 1;      // [nb + 1] first tile of a key
   uint16_t* hist = reinterpret_cast<uint16_t*>(tstart + nb + 1);  // [WARPS][nb]
   uint16_t* key_s = hist + WARPS * nb;                            // [entries of the block]
   __shared__ int sums[32], tile_total;
@@ -172,23 +175,41 @@ __global__ void __launch_bounds__(THREADS) cluster_kernel(const Plan a) {
   for (int i = tid; i < WARPS * nb / 2 + 1; i += THREADS) reinterpret_cast<uint32_t*>(hist)[i] = 0;
   __syncthreads();
   uint16_t* mine = hist + warp * nb;
-  constexpr int NONE = 0xffff;
-  for (int q = e0; q < e1; q += 32) {
-    const int i = q + lane;
-    int key = NONE;
-    if (i < e1) {
-      if (PAIRS) {
-        const int e = a.ids[(int64_t)a.row_order[i / a.k] * a.k + i % a.k];
-        key = e >= 0 && e < a.E ? e : NONE;
-      } else {
-        key = bin_of_row(a.offsets, a.slots, a.requests, i, a.n);
-        a.bins[i] = key;
+  constexpr int NONE = 0xffff, BATCH = 4;  // steps of a warp whose loads go out together
+  for (int q = e0; q < e1; q += 32 * BATCH) {
+    int key[BATCH];
+    if (MODE == ROWS) {
+#pragma unroll
+      for (int s = 0; s < BATCH; ++s) {
+        const int i = q + s * 32 + lane;
+        key[s] = i < e1 ? bin_of_row(a.offsets, a.slots, a.requests, i, a.n) : NONE;
+        if (i < e1) a.bins[i] = key[s];
       }
-      key_s[i - block0] = (uint16_t)key;
+    } else {
+      int e[BATCH], b[BATCH];
+#pragma unroll
+      for (int s = 0; s < BATCH; ++s) {
+        const int i = min(q + s * 32 + lane, e1 - 1), t = i / a.k;
+        b[s] = MODE == PAIRS ? a.row_bins[t] : a.row_order[t];
+        if (MODE == PAIRS) e[s] = a.ids[i];
+      }
+#pragma unroll
+      for (int s = 0; s < BATCH; ++s) {
+        const int i = min(q + s * 32 + lane, e1 - 1);
+        if (MODE == BY_ORDER) e[s] = a.ids[(int64_t)b[s] * a.k + i % a.k];
+      }
+#pragma unroll
+      for (int s = 0; s < BATCH; ++s)
+        key[s] = q + s * 32 + lane < e1 && e[s] >= 0 && e[s] < a.E ? (MODE == PAIRS ? e[s] * n1 + b[s] : e[s]) : NONE;
     }
-    const unsigned peers = __match_any_sync(0xffffffffu, key);
-    if (key != NONE && lane == __ffs(peers) - 1) mine[key] += (uint16_t)__popc(peers);
-    __syncwarp();
+#pragma unroll
+    for (int s = 0; s < BATCH; ++s) {
+      const int i = q + s * 32 + lane;
+      if (i < e1) key_s[i - block0] = (uint16_t)key[s];
+      const unsigned peers = __match_any_sync(0xffffffffu, key[s]);
+      if (key[s] != NONE && lane == __ffs(peers) - 1) mine[key[s]] += (uint16_t)__popc(peers);
+      __syncwarp();
+    }
   }
   __syncthreads();
   for (int b = tid; b < nb; b += THREADS) {  // each warp's first place among the block's
@@ -202,71 +223,93 @@ __global__ void __launch_bounds__(THREADS) cluster_kernel(const Plan a) {
     totals[b] = count;
   }
   cluster.sync();
-  int all = 0, before = 0;
-  if (tid < nb) {
+  constexpr int PER = CLUSTER_BINS / THREADS;  // neighbouring keys of a thread
+  int all[PER], before[PER], sum = 0, tile_sum = 0;
 #pragma unroll
-    for (int c = 0; c < MAX_CTAS; ++c) {
-      const int v = c < ctas ? cluster.map_shared_rank(totals, c)[tid] : 0;
-      all += v;
-      before += c < cta ? v : 0;
+  for (int j = 0; j < PER; ++j) {
+    const int b = tid * PER + j;
+    all[j] = before[j] = 0;
+    if (b < nb) {
+#pragma unroll
+      for (int c = 0; c < MAX_CTAS; ++c) {
+        const int v = c < ctas ? cluster.map_shared_rank(totals, c)[b] : 0;
+        all[j] += v;
+        before[j] += c < cta ? v : 0;
+      }
     }
+    sum += all[j];
+    tile_sum += (all[j] + a.tile - 1) / a.tile;
   }
   int valid, n_tiles = 0;
-  const int at = block_scan(all, sums, valid);
-  if (tid < nb) start[tid] = at + before, global[tid] = at;
-  if (tid == 0) global[nb] = valid;
-  if (PAIRS) {
-    if (cta == 0)
-      for (int b = tid; b <= nb; b += THREADS) a.expert_offsets[b] = b < nb ? (tid < nb ? at : 0) : valid;
-  } else {
-    const int tat = block_scan((all + a.tile - 1) / a.tile, sums, n_tiles);
-    if (tid < nb) tstart[tid] = tat;
-    if (tid == 0) tstart[nb] = n_tiles;
-    if (cta == 0) {
-      if (tid < nb) a.bin_offsets[tid] = at;
-      if (tid == 0) a.bin_offsets[nb] = a.entries, a.tiles[0] = n_tiles;
-    }
+  int at = block_scan(sum, sums, valid), tat = MODE == BY_ORDER ? 0 : block_scan(tile_sum, sums, n_tiles);
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int b = tid * PER + j;
+    if (b < nb) start[b] = at + before[j], global[b] = at, tstart[b] = tat;
+    at += all[j];
+    tat += (all[j] + a.tile - 1) / a.tile;
   }
+  if (tid == 0) global[nb] = valid, tstart[nb] = n_tiles;
   __syncthreads();
+  if (cta == 0) {
+    if (MODE == ROWS) {
+      for (int b = tid; b <= nb; b += THREADS) a.bin_offsets[b] = global[b];
+    } else {
+      for (int e = tid; e <= a.E; e += THREADS) a.expert_offsets[e] = global[MODE == PAIRS ? e * n1 : e];
+    }
+    if (MODE != BY_ORDER && tid == 0) a.tiles[0] = n_tiles;
+  }
   int2* list = reinterpret_cast<int2*>(a.tiles + 4);
-  if (!PAIRS) {
+  if (MODE != BY_ORDER) {
     for (int i = cta * THREADS + tid; i <= n_tiles; i += ctas * THREADS) {
-      int lo = 0, hi = nb - 1;  // the last bin whose tiles start at or before i
+      int lo = 0, hi = nb - 1;  // the last key whose tiles start at or before i
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (tstart[mid] <= i) lo = mid;
         else hi = mid - 1;
       }
-      list[i] = i == n_tiles ? make_int2(a.entries, -1) : make_int2(global[lo] + (i - tstart[lo]) * a.tile, lo < a.n ? lo : -1);
+      const int e = MODE == PAIRS ? lo / n1 : 0, bin = lo - e * n1;
+      list[i] = i == n_tiles ? make_int2(valid, -1)
+                             : make_int2(global[lo] + (i - tstart[lo]) * a.tile, bin == a.n ? -1 : MODE == PAIRS ? bin * a.E + e : bin);
     }
   }
-  for (int q = e0; q < e1; q += 32) {
-    const int i = q + lane, key = i < e1 ? (int)key_s[i - block0] : NONE;
-    const unsigned peers = __match_any_sync(0xffffffffu, key);
-    if (key != NONE) {
-      const int p = start[key] + mine[key] + __popc(peers & ((1u << lane) - 1u));
-      if (PAIRS) {
-        const int token = a.row_order[i / a.k];
-        a.pair_order[p] = (int64_t)token * a.k + i % a.k;
-        a.x_rows[p] = token;
-        const int bin = a.row_bins[token];
-        a.keys[p] = bin < a.n ? bin * a.E + key : -1 - key;  // the matrix; without an adapter a negative number per expert
-      } else {
-        a.order[p] = i;
+  for (int q = e0; q < e1; q += 32 * BATCH) {
+    int token[BATCH], bin[BATCH];
+    if (MODE == BY_ORDER) {
+#pragma unroll
+      for (int s = 0; s < BATCH; ++s) token[s] = a.row_order[min(q + s * 32 + lane, e1 - 1) / a.k];
+#pragma unroll
+      for (int s = 0; s < BATCH; ++s) bin[s] = a.row_bins[token[s]];
+    }
+#pragma unroll
+    for (int s = 0; s < BATCH; ++s) {
+      const int i = q + s * 32 + lane, key = i < e1 ? (int)key_s[i - block0] : NONE;
+      const unsigned peers = __match_any_sync(0xffffffffu, key);
+      if (key != NONE) {
+        const int p = start[key] + mine[key] + __popc(peers & ((1u << lane) - 1u));
+        if (MODE == ROWS) {
+          a.order[p] = i;
+        } else {
+          const int t = MODE == PAIRS ? i / a.k : token[s];
+          a.pair_order[p] = MODE == PAIRS ? i : (int64_t)t * a.k + i % a.k;
+          a.x_rows[p] = t;
+          if (MODE == BY_ORDER) a.keys[p] = bin[s] < a.n ? bin[s] * a.E + key : -1 - key;  // the matrix; without an adapter a negative number per expert
+        }
       }
+      __syncwarp();
+      if (key != NONE && lane == __ffs(peers) - 1) mine[key] += (uint16_t)__popc(peers);
+      __syncwarp();
     }
-    __syncwarp();
-    if (key != NONE && lane == __ffs(peers) - 1) mine[key] += (uint16_t)__popc(peers);
-    __syncwarp();
   }
-  if (PAIRS) {
+  if (MODE != ROWS)
     for (int p = valid + cta * THREADS + tid; p < a.entries; p += ctas * THREADS) a.pair_order[p] = -1, a.x_rows[p] = 0;
+  if (MODE == BY_ORDER) {
     cluster.sync();  // the positions' keys of all blocks
     const int per = (valid + ctas * THREADS - 1) / (ctas * THREADS), p0 = min((cta * THREADS + tid) * per, valid), p1 = min(p0 + per, valid);
     int starts = 0;
     for (int p = p0; p < p1; ++p) starts += p % a.tile == 0 || a.keys[p] != a.keys[p - 1];
     int total;
-    int tat = block_scan(starts, sums, total);
+    tat = block_scan(starts, sums, total);
     if (tid == 0) tile_total = total;
     cluster.sync();
     int everything = 0;
@@ -286,22 +329,22 @@ __global__ void __launch_bounds__(THREADS) cluster_kernel(const Plan a) {
   cluster.sync();  // nobody leaves while its counts may be read
 }
 
-template <bool PAIRS>
+template <int MODE>
 int launch_cluster(const Plan& a, cudaStream_t st) {
-  const int nb = PAIRS ? a.E : a.n + 1;
+  const int nb = MODE == BY_ORDER ? a.E : MODE == PAIRS ? a.E * (a.n + 1) : a.n + 1;
   int ctas = 1;
   while (ctas < MAX_CTAS && (int64_t)ctas * THREADS < a.entries) ctas *= 2;
   const int64_t run = (cdiv64(a.entries, ctas * WARPS) + 31) & ~(int64_t)31;
   const size_t smem = (size_t)(4 * nb + 2) * 4 + (size_t)WARPS * nb * 2 + 4 + (size_t)WARPS * run * 2;
-  constexpr int MOST = (4 * CLUSTER_BINS + 2) * 4 + WARPS * CLUSTER_BINS * 2 + 4 + (int)(CLUSTER_ENTRIES / MAX_CTAS) * 2;  // 113 KB
-  DST_CUDA_TRY(cudaFuncSetAttribute(cluster_kernel<PAIRS>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST));
+  constexpr int MOST = (4 * CLUSTER_BINS + 2) * 4 + WARPS * CLUSTER_BINS * 2 + 4 + (int)(CLUSTER_ENTRIES / MAX_CTAS) * 2;  // 193 KB
+  DST_CUDA_TRY(cudaFuncSetAttribute(cluster_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ctas, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr, cfg.numAttrs = 1;
-  DST_CUDA_TRY(cudaLaunchKernelEx(&cfg, cluster_kernel<PAIRS>, a));
+  DST_CUDA_TRY(cudaLaunchKernelEx(&cfg, cluster_kernel<MODE>, a));
   return DST_OK;
 }
 
@@ -446,7 +489,7 @@ extern "C" int dst_adapter_plan(const int32_t* offsets, const int32_t* slots, in
   a.offsets = offsets, a.slots = slots, a.requests = requests, a.entries = (int)rows, a.n = (int)n, a.tile = tile;
   a.order = order, a.bins = bins, a.bin_offsets = bin_offsets, a.tiles = tiles;
   if (rows <= (n < CLUSTER_BINS ? RANK_ROWS : SMALL)) return launch_small(a, st);
-  if (one_cluster(rows, n + 1)) return launch_cluster<false>(a, st);
+  if (one_cluster(rows, n + 1)) return launch_cluster<ROWS>(a, st);
   if (!workspace || workspace_bytes < dst_adapter_plan_workspace_bytes(rows, n)) return DST_ERR_BAD_ARG;
   char* w = static_cast<char*>(workspace);
   int64_t* order64 = reinterpret_cast<int64_t*>(w);
@@ -487,7 +530,8 @@ extern "C" int dst_adapter_plan_experts(const int32_t* ids, int64_t T, int top_k
     p.ids = ids, p.row_order = order, p.row_bins = bins, p.entries = (int)pairs, p.n = (int)n, p.k = top_k, p.E = (int)E, p.tile = tile;
     p.pair_order = pair_order, p.expert_offsets = offsets, p.x_rows = x_rows, p.tiles = tiles, p.keys = static_cast<int32_t*>(workspace);
     if (pairs == 0) p.ids = reinterpret_cast<const int32_t*>(tiles);  // not read: says that these are pairs
-    return small ? launch_small(p, st) : launch_cluster<true>(p, st);
+    if (small) return launch_small(p, st);
+    return E * (n + 1) <= CLUSTER_BINS ? launch_cluster<PAIRS>(p, st) : launch_cluster<BY_ORDER>(p, st);
   }
   const unsigned blocks = (unsigned)cdiv64(pairs, THREADS);
   char* w = static_cast<char*>(workspace);

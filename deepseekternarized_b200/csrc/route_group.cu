@@ -201,10 +201,13 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
   const int lane = threadIdx.x & 31, tl = lane % LPT;
   const unsigned segment = LPT == 32 ? FULL : ((1u << LPT) - 1u) << (lane - tl);
   const auto seg_max = [&](uint32_t v) {
-    if (LPT == 32) return __reduce_max_sync(FULL, v);
+    if constexpr (LPT == 32) {
+      return __reduce_max_sync(FULL, v);
+    } else {
 #pragma unroll
-    for (int off = LPT / 2; off > 0; off >>= 1) v = max(v, __shfl_xor_sync(FULL, v, off));
-    return v;
+      for (int off = LPT / 2; off > 0; off >>= 1) v = max(v, __shfl_xor_sync(FULL, v, off));
+      return v;
+    }
   };
   const auto seg_any = [&](bool v) { return (__ballot_sync(FULL, v) & segment) != 0; };
   const int64_t row = t * a.stride;

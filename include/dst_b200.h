@@ -292,7 +292,7 @@ int dst_moe_layer(const void* x_bf16, const float* weights, const int32_t* ids, 
  * each position; adapters 0 .. n-1, then the rows without one, each in row order), bins [rows] (the row's adapter, n: none),
  * bin_offsets [n + 2] (where each adapter's positions start, then those without one, then rows), tiles
  * [dst_adapter_tile_capacity(rows, n + 1, tile)], 8-byte aligned: the positions cut into tiles of at most `tile` rows of one
- * adapter. n <= 4095. Workspace: dst_adapter_plan_workspace_bytes (0 up to 1024 rows, and up to 131072 with at most 1023 adapters).
+ * adapter. n <= 4095. Workspace: dst_adapter_plan_workspace_bytes (0 up to 1024 rows, and up to 131072 with at most 2047 adapters).
  *
  * dst_adapter_plan_experts: the (token, choice) pairs of a MoE layer, ids [T, top_k], sorted by expert and inside an expert by
  * adapter, from the tokens' plan (order, bins). pair_order [T * top_k] = token * top_k + choice per position (-1 behind the

@@ -206,7 +206,7 @@ def check_plan(plan, slots, n):
 
 @gpu
 @pytest.mark.parametrize("rows,n", [(1, 1), (1, 7), (31, 3), (33, 64), (257, 1), (1000, 5), (5000, 200), (16384, 64), (16384, 1023), (16385, 9), (700, 1024),
-                                    (1024, 4000), (1025, 40), (131072, 3), (131073, 3), (2000, 1022),
+                                    (1024, 4000), (1025, 40), (131072, 3), (131073, 3), (2000, 1022), (20000, 2047), (3000, 2048), (5000, 3000),
                                     (40000, 2000), (0, 3), (0, 1500)])
 def test_plan_of_row_slots(rows, n):
     g = gen(rows + n)
@@ -232,7 +232,8 @@ def test_plan_of_requests():
 
 @gpu
 @pytest.mark.parametrize("T,k,E,n", [(1, 6, 384, 3), (7, 2, 8, 1), (8, 6, 384, 2), (64, 8, 64, 12), (130, 8, 16, 4), (300, 1, 5, 2), (3000, 8, 64, 4), (0, 2, 4, 2), (128, 8, 4096, 3),
-                                     (129, 8, 1024, 300), (129, 8, 1025, 2), (700, 6, 1100, 5), (16384, 8, 16, 2), (16385, 8, 16, 2)])
+                                     (129, 8, 1024, 300), (129, 8, 1025, 2), (700, 6, 1100, 5), (16384, 8, 16, 2), (16385, 8, 16, 2), (700, 6, 64, 40),
+                                     (129, 8, 2049, 2), (3000, 8, 512, 3), (3000, 8, 2048, 1)])
 def test_plan_of_experts(T, k, E, n):
     g = gen(T * k + E)
     slots = torch.randint(-1, n, (T,), generator=g, device=DEV)
@@ -306,7 +307,7 @@ def test_abi_argument_checks():
     assert lib.dst_adapter_plan(None, None, 4, 4, 3, 16, p, p, p, p, None, 0, None) == 1
     assert lib.dst_adapter_plan(None, p, 4, 4, 3, 16, None, p, p, p, None, 0, None) == 1
     assert lib.dst_adapter_plan(None, p, 4, 4, 3, 16, p, p, p, p + 4, None, 0, None) == 5
-    assert lib.dst_adapter_plan(None, p, 20000, 20000, 2000, 16, p, p, p, p, None, 0, None) == 1  # no workspace
+    assert lib.dst_adapter_plan(None, p, 20000, 20000, 3000, 16, p, p, p, p, None, 0, None) == 1  # no workspace
     assert lib.dst_adapter_plan_experts(p, 4, 2, 5000, p, p, 3, 16, p, p, p, p, p, 1 << 20, None) == 2
     assert lib.dst_adapter_plan_experts(p, 4000, 2, 8, p, p, 3, 16, p, p, p, p, p, 8, None) == 1
     assert lib.dst_adapter_plan_experts(p, 1 << 30, 8, 8, p, p, 3, 16, p, p, p, p, p, 1 << 20, None) == 2
