@@ -8,9 +8,10 @@
 //   weight_i = s of pick i, divided by the picks' sum + 1e-20 when renormalised (top_k > 1), times route_scale
 //
 // The picks are those of exact arithmetic. Without a bias f keeps the order of the logits, which decide by themselves; sums of two
-// scores and keys with a bias are compared in float32 where they are further apart than their rounding errors can reach, and a
-// token with a closer border is done again in 64 bits. A NaN ranks above every number (such a token goes the 64-bit way too), so
-// a token's ids are distinct and inside [0, E) whatever the logits hold.
+// scores and keys with a bias are compared in float32 where they are further apart than their rounding errors can reach. Picks that
+// are closer are told apart in 64 bits by themselves, where that takes no sum over all experts; a token with closer groups is done
+// again in 64 bits by its block. A NaN ranks above every number (such a token goes that way too), so a token's ids are distinct and
+// inside [0, E) whatever the logits hold. A token done again costs its block 4 to 7 us (256 experts), a few close picks 1.
 #include "dst_common.cuh"
 
 namespace dst {
@@ -63,30 +64,42 @@ __device__ __forceinline__ double score64(double z, double mx, double sum) {
   return sqrt(fmax(z, 0.0) + log1p(exp(-fabs(z))));  // a NaN comes through log1p
 }
 
-// A token in 64 bits by the whole block, its keys in shared memory (`keys` [E]).
+// A token in 64 bits by the whole block, its keys in shared memory (`keys` [E]). Few tokens come here, but the kernel ends with the
+// last of them: the evaluations of a thread overlap, and a lane looks at its run of keys eight at a time.
 template <int SCORE>
 __device__ __noinline__ void route_exact(const GroupRoute& a, int64_t t, uint64_t* keys, double* red) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = t * a.stride;
-  const double temp = a.temp;
+  const auto logit = [&](int e) {
+    const double v = load_logit(a, row + e);
+    return a.temp == 1.f ? v : v / (double)a.temp;
+  };
   double mx = -INFINITY, sum = 0.0;
   if (SCORE == DST_SCORE_SOFTMAX) {
-    for (int e = tid; e < a.E; e += WARPS * 32) mx = fmax(mx, (double)load_logit(a, row + e) / temp);
+    for (int e = tid; e < a.E; e += WARPS * 32) mx = fmax(mx, logit(e));
     for (int off = 16; off > 0; off >>= 1) mx = fmax(mx, __shfl_xor_sync(FULL, mx, off));
     if (lane == 0) red[warp] = mx;
     __syncthreads();
     for (int w = 0; w < WARPS; ++w) mx = fmax(mx, red[w]);
     __syncthreads();
-    for (int e = tid; e < a.E; e += WARPS * 32) sum += exp((double)load_logit(a, row + e) / temp - mx);
+    for (int e = tid; e < a.E; e += WARPS * 32) sum += exp(logit(e) - mx);
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(FULL, sum, off);
     if (lane == 0) red[warp] = sum;
     __syncthreads();
     sum = 0.0;
     for (int w = 0; w < WARPS; ++w) sum += red[w];
   }
-  for (int e = tid; e < a.E; e += WARPS * 32) {
-    const double s = score64<SCORE>((double)load_logit(a, row + e) / temp, mx, sum);
-    keys[e] = order_of(a.bias ? s + (double)a.bias[e] : s);
+  for (int e0 = tid; e0 < a.E; e0 += 4 * WARPS * 32) {
+    double s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = logit(min(e0 + i * WARPS * 32, a.E - 1));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = score64<SCORE>(s[i], mx, sum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = e0 + i * WARPS * 32;
+      if (e < a.E) keys[e] = order_of(a.bias ? s[i] + (double)a.bias[e] : s[i]);
+    }
   }
   __syncthreads();
   if (warp == 0) {  // a group is a matter of 32 >> wide neighbouring lanes, each with its own run of experts
@@ -94,13 +107,23 @@ __device__ __noinline__ void route_exact(const GroupRoute& a, int64_t t, uint64_
     while ((1 << wide) < a.groups) ++wide;
     const int lanes = 32 >> wide, group = lane / lanes, run = (a.size + lanes - 1) / lanes, first = (lane % lanes) * run;
     const int n = group < a.groups ? min(run, a.size - first) : 0, id0 = group * a.size + first;
-    uint64_t m1 = 0, m2 = 0;
-    for (int j = 0; j < n; ++j) {
-      const uint64_t k = keys[id0 + j];
-      if (k > m1) m2 = m1, m1 = k;
-      else if (k > m2) m2 = k;
-    }
-    const uint64_t own = m1;
+    const auto two_of = [&](uint64_t& m1, uint64_t& m2, int& at) {  // the two largest of the lane's keys, and where the first is
+      m1 = m2 = 0, at = 0;
+      for (int j0 = 0; j0 < n; j0 += 8) {
+        uint64_t k[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k[i] = j0 + i < n ? keys[id0 + j0 + i] : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (k[i] > m1) m2 = m1, m1 = k[i], at = j0 + i;
+          else if (k[i] > m2) m2 = k[i];
+        }
+      }
+    };
+    uint64_t m1, m2;
+    int at;
+    two_of(m1, m2, at);
+    uint64_t best = m1;  // the lane's largest that is left
     for (int off = 1; off < lanes; off <<= 1) {
       const uint64_t o1 = __shfl_xor_sync(FULL, m1, off), o2 = __shfl_xor_sync(FULL, m2, off);
       if (o1 > m1) m2 = m1 > o2 ? m1 : o2, m1 = o1;
@@ -112,33 +135,24 @@ __device__ __noinline__ void route_exact(const GroupRoute& a, int64_t t, uint64_
       const uint64_t o = __shfl_sync(FULL, g, h * lanes);
       better += o > g || (o == g && h < group);
     }
-    const bool keep = group < a.groups && better < a.kept;
-    uint64_t best = keep ? own : 0;  // the lane's largest that is left
-    double my_w = 0.0, wsum = 0.0;
+    if (!(group < a.groups && better < a.kept)) best = 0;
     int my_id = 0;
     for (int r = 0; r < a.top_k; ++r) {
-      uint64_t top = best;
-      for (int off = 16; off > 0; off >>= 1) {
-        const uint64_t o = __shfl_xor_sync(FULL, top, off);
-        top = o > top ? o : top;
-      }
-      const int win = __ffs(__ballot_sync(FULL, best == top)) - 1;
-      int at = 0;
+      // the largest of the warp: its upper halves first, its lower ones among those that share it
+      const uint32_t hi = __reduce_max_sync(FULL, (uint32_t)(best >> 32));
+      const uint32_t lo = __reduce_max_sync(FULL, (uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+      const int win = __ffs(__ballot_sync(FULL, best == (((uint64_t)hi << 32) | lo))) - 1;
+      const int id = __shfl_sync(FULL, id0 + at, win);
+      if (lane == r) my_id = id;
       if (lane == win) {
-        uint64_t next = 0;
-        bool taken = false;
-        for (int j = 0; j < n; ++j) {
-          const uint64_t k = keys[id0 + j];
-          if (k == best && !taken) keys[id0 + j] = 0, at = id0 + j, taken = true;
-          else if (k > next) next = k;
-        }
-        best = next;
+        keys[id0 + at] = 0;
+        uint64_t unused;
+        two_of(best, unused, at);
       }
-      at = __shfl_sync(FULL, at, win);
-      if (lane == r) my_id = at;
+      __syncwarp();
     }
-    if (lane < a.top_k) my_w = score64<SCORE>((double)load_logit(a, row + my_id) / temp, mx, sum);
-    wsum = my_w;
+    const double my_w = lane < a.top_k ? score64<SCORE>(logit(min(my_id, a.E - 1)), mx, sum) : 0.0;
+    double wsum = my_w;
     for (int off = 4; off > 0; off >>= 1) wsum += __shfl_xor_sync(FULL, wsum, off);
     if (lane < a.top_k) {
       a.weights[t * a.top_k + lane] = (float)((a.renorm && a.top_k > 1 ? my_w / (wsum + 1e-20) : my_w) * (double)a.scale);
@@ -224,7 +238,13 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
   } else {
-    for (int j = 0; j < n; ++j) own[j] = __float_as_uint(load_logit(a, row + id0 + j));
+    for (int j0 = 0; j0 < n; j0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = load_logit(a, row + id0 + min(j0 + i, n - 1));
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) *reinterpret_cast<float4*>(own + j0 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    }
   }
   // The lane's numbers in blocks of eight. A logit is negated under a negative temperature: experts rank by it as they do by their
   // scores. zmax, zmin and `special` (a NaN from anything that is not finite) come out of the first pass.
@@ -405,6 +425,7 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
   float zi = pick ? load_logit(a, row + id) : 0.f;
   if (flip) zi = -zi;
 
+  bool settled = false;  // written below already
   if (a.bias) {
     // picks in the right order: each further above the next than both errors, or of the same logit and bias
     const float key = value_of(number), b = pick ? a.bias[id] : 0.f;
@@ -417,7 +438,8 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
     const int first_from = __shfl_sync(FULL, from, 0, LPT);
     const bool one_lane = !seg_any(pick && from != first_from);
     const bool any_unsure = seg_any(unsure);
-    again = again || any_unsure || (a.top_k == 8 && a.chunk > 8 && one_lane);
+    again = again || (a.top_k == 8 && a.chunk > 8 && one_lane);
+    bool near_picks = any_unsure;
     const bool border = left && !(last - value_of(left) > last_tol);
     if (__any_sync(FULL, border && !again)) {  // equal logits and biases at the border are no matter
       const float last_z = __shfl_sync(FULL, zi, a.top_k - 1, LPT), last_b = __shfl_sync(FULL, b, a.top_k - 1, LPT);
@@ -431,7 +453,60 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
           }
         }
       const bool any_other = seg_any(other);
-      again = again || any_other;
+      near_picks = near_picks || any_other;
+    }
+    near_picks = near_picks && !again;
+    if (SCORE == DST_SCORE_SOFTMAX) {
+      again = again || near_picks;  // the sum of all scores would be needed in 64 bits
+    } else if (__any_sync(FULL, near_picks)) {
+      // The picks and, of each lane, the next one where it is as near as the last pick, in 64 bits: each takes the place of its rank
+      // among them. Two such in a lane, or a list that has run out behind the first: the other form.
+      const bool extra = near_picks && top[0] && !(last - value_of(top[0]) > last_tol);
+      const bool any_more = seg_any(extra && (top[1] ? !(last - value_of(top[1]) > last_tol) : n > 8));
+      again = again || any_more;
+      int skip = 0, next = 0;  // the extra one is the lane's first of its number behind the lane's picks of that number
+      for (int r = 0; r < a.top_k; ++r) {
+        const uint32_t o = __shfl_sync(FULL, number, r, LPT);
+        const int f = __shfl_sync(FULL, from, r, LPT);
+        skip += o == top[0] && f == tl;
+      }
+      if (extra)
+        for (int j = 0; j < n; ++j)
+          if (own[j] == top[0] && skip-- == 0) next = j;
+      const int extra_id = id0 + next;
+      const float extra_z = extra ? load_logit(a, row + extra_id) : 0.f;
+      const auto key64 = [&](float z, int e) {
+        const double v = a.temp == 1.f ? (double)z : (double)z / (double)a.temp;
+        return order_of(score64<SCORE>(v, 0.0, 1.0) + (double)a.bias[e]);
+      };
+      const uint64_t own_key = pick ? key64(flip ? -zi : zi, id) : 0, extra_key = extra ? key64(extra_z, extra_id) : 0;
+      int own_rank = 0, extra_rank = 0;
+      const auto against = [&](uint64_t key, int e) {
+        own_rank += key > own_key || (key == own_key && e < id);
+        extra_rank += key > extra_key || (key == extra_key && e < extra_id);
+      };
+      for (int r = 0; r < a.top_k; ++r) {
+        const uint64_t k = __shfl_sync(FULL, own_key, r, LPT);
+        const int e = __shfl_sync(FULL, id, r, LPT);
+        against(k, e);
+      }
+      for (int r = 0; r < LPT; ++r) {
+        const uint64_t k = __shfl_sync(FULL, extra_key, r, LPT);
+        const int e = __shfl_sync(FULL, extra_id, r, LPT);
+        if (k) against(k, e);
+      }
+      settled = near_picks && !again;
+      const bool own_in = pick && own_rank < a.top_k, extra_in = extra && extra_rank < a.top_k;
+      const float extra_t = flip ? -extra_z : extra_z, own_t = inv_temp == 1.f ? zi : zi / fabsf(a.temp);
+      float w1 = own_in ? score_of<SCORE>(own_t) : 0.f, w2 = extra_in ? score_of<SCORE>(inv_temp == 1.f ? extra_t : extra_t / fabsf(a.temp)) : 0.f;
+      if (a.renorm && a.top_k > 1) {
+        float wsum = w1 + w2;
+#pragma unroll
+        for (int off = LPT / 2; off > 0; off >>= 1) wsum += __shfl_xor_sync(FULL, wsum, off);
+        w1 = w1 / (wsum + 1e-20f), w2 = w2 / (wsum + 1e-20f);
+      }
+      if (settled && valid && own_in) a.weights[t * a.top_k + own_rank] = w1 * a.scale, a.ids[t * a.top_k + own_rank] = id;
+      if (settled && valid && extra_in) a.weights[t * a.top_k + extra_rank] = w2 * a.scale, a.ids[t * a.top_k + extra_rank] = extra_id;
     }
   }
   const float zt = inv_temp == 1.f ? zi : zi / fabsf(a.temp);
@@ -446,7 +521,7 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
     for (int off = 4; off > 0; off >>= 1) wsum += __shfl_xor_sync(FULL, wsum, off);
     w = w / (wsum + 1e-20f);
   }
-  if (pick && valid && !again) {
+  if (pick && valid && !again && !settled) {
     a.weights[t * a.top_k + tl] = w * a.scale;
     a.ids[t * a.top_k + tl] = id;
   }
@@ -492,11 +567,14 @@ int launch(GroupRoute a, cudaStream_t st) {
 
 template <int SCORE>
 int launch_for(const GroupRoute& a, cudaStream_t st) {
-  // A warp for each token as long as all of them run at once; then several tokens a warp, which share the steps across lanes.
-  // 384 experts in eight groups, top-6 (8) with sums and a bias, us for 777 / 16 384 tokens: a warp each 5.6 / 40.7 (44), two a warp
-  // 7.1 / 32.9 (36), four a warp 10.4 / 33.5 (35); without a bias and by the largest (top-8) two 18, four 14
-  if (a.groups > 16 || a.T <= 32 * (int64_t)sm_count()) return launch<SCORE, 32>(a, st);
-  if (a.groups > 8 || a.E > 512) return launch<SCORE, 16>(a, st);
+  // A warp for each token where that is a dozen of them a multiprocessor; then several tokens a warp, which share the steps across
+  // lanes. Eight groups, us for 777 / 2000 / 4736 / 16 384 tokens: 384 experts, top-6, square roots of softplus, sums and a bias: a
+  // warp each 8.5 / 10.8 / 17.2 / 38.2, two a warp 9.2 / 10.4 / 15.5 / 28.4, four 11.9 / 12.9 / 18.6 / 27.3; 256 experts, top-8,
+  // sigmoid, sums and a bias: 6.5 / 8.8 / 13.6 / 26.6, 7.2 / 9.0 / 12.0 / 21.5, 7.3 / 8.9 / 11.8 / 19.4; by the largest, without a
+  // bias: 4.4 / 5.6 / 8.5 / 19.5, 4.6 / 5.3 / 6.9 / 15.0, 4.6 / 4.8 / 5.7 / 11.3
+  const int64_t sms = sm_count();
+  if (a.groups > 16 || a.T <= 12 * sms) return launch<SCORE, 32>(a, st);
+  if (a.groups > 8 || a.E > 512 || a.T <= 32 * sms) return launch<SCORE, 16>(a, st);
   return launch<SCORE, 8>(a, st);
 }
 

@@ -131,6 +131,28 @@ def test_route_groups_border_cases_are_decided_in_64_bits(score):
 
 
 @gpu
+@pytest.mark.parametrize("T,E,groups,kept,k", [(5000, 128, 1, 1, 7), (5000, 128, 1, 1, 8), (5000, 128, 1, 1, 5), (5000, 256, 8, 8, 8), (9, 256, 8, 3, 7),
+                                               (30, 512, 1, 1, 8)])
+@pytest.mark.parametrize("score", ["sigmoid", "sqrtsoftplus"])
+def test_route_groups_near_picks(T, E, groups, kept, k, score):
+    """Up to nine keys that differ by less than their rounding, at the border of the picks and inside it: anywhere, or all of them
+    neighbours, so that one lane holds more of them than its list; far ones above and below."""
+    g = gen(E + k)
+    logits = torch.rand(T, E, generator=g, device=DEV) - 4.0
+    near = (torch.full((T, 9), 1.25, device=DEV).view(torch.int32) + torch.randint(0, 5, (T, 9), generator=g, device=DEV).to(torch.int32)).view(torch.float32)
+    count = 2 + torch.randint(0, 8, (T, 1), generator=g, device=DEV)
+    at = torch.rand(T, E, generator=g, device=DEV).argsort(dim=-1)[:, :9]
+    run = 16 * torch.randint(0, E // 16, (T, 1), generator=g, device=DEV) + torch.arange(9, device=DEV)
+    at = torch.where(torch.arange(T, device=DEV)[:, None] % 2 == 0, at, run)
+    near = torch.where(torch.arange(9, device=DEV) < count, near, torch.rand(T, 9, generator=g, device=DEV) + 2.0)
+    logits.scatter_(1, at, near)
+    bias = torch.zeros(E, device=DEV)
+    bias[::5] = 2.0 ** -26
+    check_route(logits, k, 1.0, True, score, bias, 1.0, groups, kept, "max")
+    check_route(-1.5 * logits, k, 1.0, False, score, bias, -1.5, groups, kept, "max")
+
+
+@gpu
 @pytest.mark.parametrize("score", ["sigmoid", "softmax", "sqrtsoftplus"])
 def test_route_groups_infinities_and_nan(score):
     g = gen(11)
