@@ -15,8 +15,9 @@ Cut cut_of(int64_t max_tiles, int tile, int64_t K_padded, int64_t N, int rank_pa
   const int64_t sms = sm_count(), blocks = max_tiles * (tile / 16);
   Cut cut{0, 8, 1, 1, 0};
   // Up to 48 blocks the cluster's one launch costs the host 5 us less (11 against 16 a call) and the device as much: 1 row of 4096 x
-  // 4096 4.2 us against 4.1, 333 rows 8.0 against 8.2, 48 pairs (rank 16 twice) 13.1 against 14.4 with their plan; 64 rows of 37 adapters (53 blocks) through 11008 x 4096 14.9 against 11.2
-  if (blocks <= 48) {
+  // 4096 4.2 us against 4.1, 333 rows 8.0 against 8.2, 48 pairs (rank 16 twice) 13.1 against 14.4 with their plan; 64 rows of 37
+  // adapters (53 blocks) through 11008 x 4096 14.9 against 11.2. A cluster takes tiles of 16 rows only.
+  if (tile == 16 && blocks <= 48) {
     cut.ctas = 1;
     while (cut.ctas < ADAPTER_MAX_CTAS && max_tiles * cut.ctas * 2 <= 2 * sms) cut.ctas *= 2;
     return cut;
@@ -62,12 +63,15 @@ extern "C" int dst_adapter_apply(const dst_adapters* w, const dst_adapter_rows* 
       (w->dtype != DST_ACT_BF16 && w->dtype != DST_ACT_F16) || w->K <= 0 || w->N <= 0 ||
       w->matrices_per_slot <= 0 || plan->max_tiles < 0)
     return DST_ERR_BAD_ARG;
-  if (w->parts < 1 || w->N % w->parts != 0 || w->K_padded < w->K || w->K_padded % 64 != 0 || x_stride < w->K || out_stride < w->N ||
-      (base && base_stride < w->N) || plan->max_tiles > 0x00ffffff || plan->positions < 0 || w->N > (1 << 24) || w->K_padded > (1 << 24) || (plan->tile != 16 && plan->tile != 128))
+  if (w->parts < 1 || w->N % w->parts != 0 || w->N > (1 << 24) || w->K > (1 << 24) || w->K_padded != cdiv64(w->K, 64) * 64 || x_stride < w->K ||
+      out_stride < w->N || (base && base_stride < w->N) || plan->max_tiles > 0x00ffffff || plan->positions < 0 ||
+      (plan->tile != 16 && plan->tile != 128))
     return DST_ERR_BAD_SHAPE;
   if (plan->max_tiles == 0) return DST_OK;
   if (!w->a || !w->b || !w->scale || !w->ranks || !plan->tiles || !x || !out) return DST_ERR_BAD_ARG;
-  if (((reinterpret_cast<uintptr_t>(w->a) | reinterpret_cast<uintptr_t>(w->b)) & 15) != 0 || (reinterpret_cast<uintptr_t>(plan->tiles) & 7) != 0)
+  const auto off = [](const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size != 0; };
+  if (off(w->a, 16) || off(w->b, 16) || off(plan->tiles, 8) || off(w->scale, 4) || off(w->ranks, 4) || off(plan->rows, 4) ||
+      off(plan->x_rows, 4) || off(x, 2) || off(base, base_dtype == DST_OUT_F32 ? 4 : 2) || off(out, out_dtype == DST_OUT_F32 ? 4 : 2))
     return DST_ERR_ALIGNMENT;
   AdapterCall c{};
   c.x = x, c.x_stride = x_stride, c.x_rows = plan->x_rows, c.rows = plan->rows, c.tiles = plan->tiles;
@@ -84,7 +88,8 @@ extern "C" int dst_adapter_apply(const dst_adapters* w, const dst_adapter_rows* 
     else if (out_dtype == own && (!base || base_dtype == own)) c.kind = base ? 2 : 3;
   }
   const Cut cut = cut_of(plan->max_tiles, plan->tile, w->K_padded, w->N, w->rank_padded, c.x_vec && c.kind >= 0);
-  c.sub = plan->tile / 16, c.shared = cut.shared, c.ctas = cut.ctas, c.share = cut.share, c.k_splits = cut.k_splits, c.splits = cut.columns, c.positions = plan->positions, c.h = static_cast<float*>(workspace);
+  c.sub = plan->tile / 16, c.shared = cut.shared, c.ctas = cut.ctas, c.share = cut.share, c.k_splits = cut.k_splits, c.splits = cut.columns;
+  c.positions = plan->positions, c.h = static_cast<float*>(workspace);
   if (!cut.ctas) {
     if (!workspace || workspace_bytes < dst_adapter_workspace_bytes(w, plan)) return DST_ERR_BAD_ARG;
     if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return DST_ERR_ALIGNMENT;

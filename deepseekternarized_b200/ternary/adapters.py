@@ -139,12 +139,11 @@ class ExpertPlan:
         self._buf = torch.empty(words, dtype=torch.int64, device=dev)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         base, src = self._buf.data_ptr(), plan._buf.data_ptr()
-        p_offsets = base + 8 * P
-        self._tiles = p_offsets + 8 * (n_experts + 1)
-        self._x_rows = self._tiles + 8 * tiles
+        self._at = P + n_experts + 1, P + n_experts + 1 + tiles  # tiles, x rows
+        p_offsets, p_tiles, p_x_rows = base + 8 * P, base + 8 * self._at[0], base + 8 * self._at[1]
         with kb._guard(dev):
             _lib.check(lib.dst_adapter_plan_experts(ids.data_ptr(), T, k, n_experts, src + 4 * plan._at[0], src + 4 * plan._at[1], n, self.tile,
-                                                    base, p_offsets, self._x_rows, self._tiles, ws.data_ptr() if ws is not None else None,
+                                                    base, p_offsets, p_x_rows, p_tiles, ws.data_ptr() if ws is not None else None,
                                                     ws_bytes, kb._stream(ids)))
         self._order = self._offsets = None
         self._c = [None, None]
@@ -153,7 +152,9 @@ class ExpertPlan:
         """The C struct of the pairs with x rows of the tokens or of the pairs, made when a projection asks for it first."""
         c = self._c[pair_rows]
         if c is None:
-            c = self._c[pair_rows] = ctypes.byref(_lib.AdapterRowsC(None, None if pair_rows else self._x_rows, self._tiles, self.max_tiles, self.n_rows, self.tile))
+            base = self._buf.data_ptr()
+            c = self._c[pair_rows] = ctypes.byref(_lib.AdapterRowsC(None, None if pair_rows else base + 8 * self._at[1], base + 8 * self._at[0],
+                                                                    self.max_tiles, self.n_rows, self.tile))
         return c
 
     @property
@@ -268,6 +269,9 @@ class LowRankAdapters:
             raise RuntimeError("the result is float32, bf16 or fp16 [rows, N]")
         else:
             out_stride = max(out.stride(0), N)
+            in_place = base is not None and (base.data_ptr(), base.dtype, base_stride) == (out.data_ptr(), out.dtype, out_stride)
+            if _meet(out, x) or (base is not None and not in_place and _meet(out, base)):
+                raise RuntimeError("the result may share memory with the base alone, and only as the base itself")
         out_code = kb._OUT.get(out.dtype)
         if out_code is None:
             raise RuntimeError("the result is float32, bf16 or fp16 [rows, N]")
@@ -291,3 +295,15 @@ class LowRankAdapters:
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """Rows of neighbouring elements, one behind the other at any distance; anything else is copied."""
     return t if (t.stride(1) == 1 or t.size(1) == 1) and (t.stride(0) >= t.size(1) or t.size(0) == 1) else t.contiguous()
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of rows can share bytes. Column ranges of one wider tensor do not."""
+    if not a.numel() or not b.numel():
+        return False
+    (p, wa, sa, ea), (q, wb, sb, eb) = ((t.data_ptr(), t.size(1) * t.element_size(), t.stride(0) * t.element_size(),
+                                         ((t.size(0) - 1) * t.stride(0) + t.size(1)) * t.element_size()) for t in (a, b))
+    if p + ea <= q or q + eb <= p:
+        return False
+    d = (q - p) % sa if sa else 0
+    return sa != sb or a.size(0) == 1 or b.size(0) == 1 or d < wa or sa - d < wb

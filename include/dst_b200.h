@@ -317,7 +317,7 @@ int dst_adapter_plan_experts(const int32_t* ids, int64_t T, int top_k, int64_t E
  * x); 31 more rows behind the last matrix of B can be read. Part p of the columns (N / parts each) takes rows p * rank_padded ..
  * of A. matrices_per_slot: matrices of one adapter (experts; 1 beside a dense projection), adapter a = m / matrices_per_slot with
  * the rank ranks[a] <= rank_padded; what lies behind it is finite and counts for nothing (rank 0: the base alone).
- * rank_padded 16, 32, 64 or 128; parts 1 or 2 with parts * rank_padded <= 128; K_padded a multiple of 64.
+ * rank_padded 16, 32, 64 or 128; parts 1 or 2 with parts * rank_padded <= 128; K_padded: K rounded up to a multiple of 64.
  * rows / x_rows: base / out row and x row of a position (NULL: the position). base (DST_OUT_* type) may be NULL (zeros) or the
  * same rows as out; x may not overlap out. Strides in elements. positions: rows of the plan (pairs of a layer). Workspace (16-byte
  * aligned): dst_adapter_workspace_bytes, by sizes and rank_padded, parts, tile alone; 0 for few tiles.

@@ -9,6 +9,8 @@ values: (K / 16 + 64 + rank) * 2^-22 + pieces. base + product is one float32 rou
 
 from __future__ import annotations
 
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -342,8 +344,9 @@ def test_abi_argument_checks():
 
     assert apply(plan=dict(max_tiles=0)) == _lib.OK
     for kw, want in ((dict(w=dict(a=None)), 1), (dict(w=dict(ranks=None)), 1), (dict(w=dict(dtype=2)), 1), (dict(w=dict(K=0)), 1), (dict(bt=3), 1), (dict(ot=-1), 1),
-                     (dict(x=None), 1), (dict(out=None), 1), (dict(w=dict(parts=3)), 2), (dict(w=dict(K_padded=32)), 2), (dict(w=dict(K_padded=96)), 2),
-                     (dict(xs=63), 2), (dict(bs=63), 2), (dict(os_=63), 2), (dict(w=dict(a=p + 2)), 5), (dict(plan=dict(max_tiles=400, positions=6400), ws=None), 1),
+                     (dict(x=None), 1), (dict(out=None), 1), (dict(w=dict(parts=3)), 2), (dict(w=dict(K_padded=32)), 2), (dict(w=dict(K_padded=96)), 2), (dict(w=dict(K_padded=128)), 2),
+                     (dict(xs=63), 2), (dict(bs=63), 2), (dict(os_=63), 2), (dict(w=dict(a=p + 2)), 5), (dict(x=p + 1), 5), (dict(base=p + 2), 5), (dict(out=p + 1), 5),
+                     (dict(plan=dict(rows=p + 2)), 5), (dict(plan=dict(max_tiles=400, positions=6400), ws=None), 1),
                      (dict(plan=dict(max_tiles=400, positions=6400), wsb=6400), 1), (dict(plan=dict(max_tiles=400, positions=6400), ws=p + 8), 5),
                      (dict(plan=dict(tile=48)), 2), (dict(plan=dict(tiles=p + 4)), 5),
                      (dict(w=dict(rank_padded=24)), 4), (dict(w=dict(rank_padded=128, parts=2)), 4)):
@@ -444,6 +447,141 @@ def test_adapters_of_long_prompts(rows, K, N, r):
     slots = torch.tensor([1, -1, 0, 1, 2], device=DEV)[torch.arange(rows, device=DEV) * 5 // rows]
     check_linear(x, slots, A, B, scale, ad, torch.randn(rows, N, generator=g, device=DEV), BF16)
     check_linear(x, slots, A, B, scale, ad, torch.randn(rows, N, generator=g, device=DEV), F32)
+
+
+def some_slots(rows, n, g):
+    """Runs of rows of one adapter or none, from one row to a quarter of the batch."""
+    cuts = torch.randint(0, rows, (6,), generator=g, device=DEV)
+    return torch.randint(-1, n, (7,), generator=g, device=DEV)[(torch.arange(rows, device=DEV)[:, None] >= cuts).sum(-1)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype,base,out", [(BF16, F32, BF16), (BF16, F32, F32), (BF16, BF16, BF16), (F16, F32, F16), (F16, F16, F16), (F16, F32, F32),
+                                            (BF16, None, None), (F16, None, None), (BF16, F16, F32)])
+@pytest.mark.parametrize("rows,r", [(900, 8), (900, 20), (900, 64), (900, 100), (3100, 16), (3100, 64), (3100, 128)])
+def test_adapters_of_many_rows(rows, r, dtype, base, out):
+    """More blocks of rows than a cluster takes; from 2960 rows on in tiles of 128, which share A and B at the higher ranks."""
+    K, N = 320, 264
+    A, B, scale, ad = make(2, K, N, r, dtype, rows)
+    g = gen(rows + r)
+    x = torch.randn(rows, K, generator=g, device=DEV).to(dtype)
+    slots = some_slots(rows, 2, g)
+    b = torch.randn(rows, N, generator=g, device=DEV).to(base) if base else None
+    y = check_linear(x, slots, A, B, scale, ad, b, out)
+    if b is not None:
+        assert torch.equal(y[slots < 0], b[slots < 0].to(y.dtype))
+        if y.dtype == b.dtype:
+            assert torch.equal(ad(x, AdapterPlan(slots, 2), base=b, out=b), y)
+
+
+@gpu
+@pytest.mark.parametrize("K,N", [(1, 1), (7, 3), (33, 31), (64, 33), (129, 200), (1000, 70), (2049, 513)])
+@pytest.mark.parametrize("rows", [850, 2970])
+def test_adapters_of_many_rows_and_odd_sizes(rows, K, N):
+    for dtype, out, r in ((BF16, BF16, 5), (F16, F32, 20), (BF16, F32, 64), (F16, F16, 128)):
+        A, B, scale, ad = make(2, K, N, r, dtype, K + N)
+        g = gen(K)
+        x = torch.randn(rows, K, generator=g, device=DEV).to(dtype)
+        check_linear(x, some_slots(rows, 2, g), A, B, scale, ad, torch.randn(rows, N, generator=g, device=DEV), out)
+
+
+@gpu
+@pytest.mark.parametrize("N,r", [(128, 8), (66, 16), (6, 3), (640, 64), (200, 32), (400, 50)])
+@pytest.mark.parametrize("rows", [900, 3000])
+def test_adapters_of_many_rows_in_two_parts(rows, N, r):
+    A, B, scale, ad = make(2, 160, N, r, BF16, N, parts=2)
+    g = gen(N)
+    x = torch.randn(rows, 160, generator=g, device=DEV).to(BF16)
+    for out in (BF16, F32):
+        check_linear(x, some_slots(rows, 2, g), A, B, scale, ad, torch.randn(rows, N, generator=g, device=DEV), out)
+
+
+@gpu
+@pytest.mark.parametrize("rows,r", [(900, 8), (900, 64), (3000, 8), (3000, 64), (3000, 128)])
+def test_adapters_of_many_rows_at_any_stride(rows, r):
+    K, N = 200, 168
+    A, B, scale, ad = make(2, K, N, r, BF16, 1)
+    g = gen(2)
+    slots = some_slots(rows, 2, g)
+    for width, off in ((24, 0), (24, 8), (24, 3), (25, 1)):
+        x = torch.randn(rows, K + width, generator=g, device=DEV).to(BF16)[:, off:off + K]
+        base = torch.randn(rows, N + width, generator=g, device=DEV)[:, off:off + N]
+        y = check_linear(x, slots, A, B, scale, ad, base, BF16)
+        out = torch.full((rows, N + 40), 7.0, dtype=BF16, device=DEV)
+        ad(x, AdapterPlan(slots, 2), base=base, out=out[:, off:off + N])
+        assert torch.equal(out[:, off:off + N], check_linear(x, slots, A, B, scale, ad, base, BF16, out=out[:, off:off + N]))
+        assert torch.allclose(out[:, off:off + N].float(), y.float(), rtol=2.0 ** -7, atol=2.0 ** -7)  # two forms of one sum
+        assert bool((out[:, off + N:] == 7).all()) and bool((out[:, :off] == 7).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,r", [(900, 16), (3000, 64)])
+def test_many_rows_keep_to_themselves(rows, r, dtype):
+    """NaNs and infinities in some rows leave the others as they were; a second call gives the same."""
+    A, B, scale, ad = make(2, 256, 128, r, dtype, 3)
+    g = gen(6)
+    x = torch.randn(rows, 256, generator=g, device=DEV).to(dtype)
+    base = torch.randn(rows, 128, generator=g, device=DEV)
+    slots = torch.randint(-1, 2, (rows,), generator=g, device=DEV)
+    plan = AdapterPlan(slots, 2)
+    y = ad(x, plan, base=base, out_dtype=dtype)
+    assert torch.equal(ad(x, plan, base=base, out_dtype=dtype), y)
+    bad, worse = torch.arange(rows, device=DEV) % 5 == 2, torch.arange(rows, device=DEV) % 7 == 3
+    x[bad], base[worse] = torch.nan, torch.inf
+    z = ad(x, plan, base=base, out_dtype=dtype)
+    fine = ~worse & (~bad | (slots < 0))
+    assert torch.equal(z[fine], y[fine])
+    assert bool(z[bad & (slots >= 0)].isnan().all()) and bool((z[worse & ~bad] == torch.inf).all())
+
+
+@gpu
+@pytest.mark.parametrize("r", [8, 64])
+def test_high_tiles_of_few_rows(r, monkeypatch):
+    """A plan may be cut into tiles of 128 rows whatever its size."""
+    from deepseekternarized_b200.ternary import adapters as mod
+
+    def high(rows, n):
+        lib = _lib.load()
+        at = int(lib.dst_adapter_tile_capacity(rows, n + 1, 128))
+        return 128, min(rows, -(-rows // 128) + n + 1), at, at + rows, at + 2 * rows, int(lib.dst_adapter_plan_workspace_bytes(rows, n))
+
+    monkeypatch.setattr(mod, "_plan_sizes", high)
+    A, B, scale, ad = make(2, 96, 64, r, BF16, 1)
+    g = gen(3)
+    for rows in (1, 40, 300):
+        x = torch.randn(rows, 96, generator=g, device=DEV).to(BF16)
+        check_linear(x, some_slots(rows, 2, g), A, B, scale, ad, torch.randn(rows, 64, generator=g, device=DEV), BF16)
+
+
+@gpu
+def test_results_may_share_memory_with_the_base_alone():
+    _, _, _, ad = make(1, 32, 32, 4, BF16, 1)
+    plan, wide = AdapterPlan(torch.zeros(6, dtype=torch.int32, device=DEV), 1), torch.zeros(7, 64, dtype=BF16, device=DEV)
+    x, base = wide[:6, :32], wide[:6, 32:]
+    ad(x, plan, base=base, out=base)  # neighbours in one tensor
+    for kw in (dict(base=base, out=x), dict(base=base, out=wide[1:, 32:]), dict(base=base, out=wide[:6, 16:48]),
+               dict(base=torch.zeros(6, 32, device=DEV), out=wide[1:, :32])):
+        with pytest.raises(RuntimeError, match="share memory"):
+            ad(x, plan, **kw)
+    b = torch.zeros(6, 32, device=DEV)
+    with pytest.raises(RuntimeError, match="share memory"):
+        ad(x, plan, base=b, out=b.view(BF16)[:, :32])
+
+
+@gpu
+def test_copies_of_plans():
+    A, B, scale, ad = make(2, 64, 32, 4, BF16, 1, experts=4)
+    g = gen(8)
+    x = torch.randn(9, 64, generator=g, device=DEV).to(BF16)
+    plan = AdapterPlan(torch.randint(-1, 2, (9,), generator=g, device=DEV), 2)
+    pairs = plan.for_experts(torch.randint(0, 4, (9, 2), generator=g, device=DEV), 4)
+    copied = copy.deepcopy(pairs)
+    assert copied._rows_c(False)._obj.tiles != pairs._rows_c(False)._obj.tiles
+    base = torch.randn(18, 32, generator=g, device=DEV)
+    assert torch.equal(ad(x, copied, base=base), ad(x, pairs, base=base))
+    with pytest.raises((TypeError, ValueError)):  # its copy would read the first one's memory
+        copy.deepcopy(ad)
 
 
 @gpu
@@ -558,7 +696,8 @@ def test_adapter_refusals():
 # ------------------------------------------------------------------------------------------------- adapters of experts
 @gpu
 @pytest.mark.parametrize("T,k,E,n,K,N,r,parts", [(1, 4, 16, 2, 128, 256, 16, 2), (9, 3, 8, 3, 256, 128, 8, 1), (200, 4, 8, 2, 64, 96, 32, 2),
-                                                 (600, 2, 4, 3, 96, 72, 16, 1), (33, 2, 6, 2, 50, 34, 4, 2)])
+                                                 (600, 2, 4, 3, 96, 72, 16, 1), (33, 2, 6, 2, 50, 34, 4, 2), (1600, 2, 2, 2, 96, 128, 64, 2),
+                                                 (1600, 2, 2, 2, 90, 100, 64, 1)])
 @pytest.mark.parametrize("pair_rows", [False, True])
 def test_adapters_of_experts(T, k, E, n, K, N, r, parts, pair_rows):
     A, B, scale, ad = make(n, K, N, r, BF16, T, experts=E, parts=parts)
@@ -694,17 +833,21 @@ def test_adapted_standard_layer_and_dropped_ids():
     weights, ids = v4.route(logits)
     ids[2, 1], ids[5, 0] = -1, E
     torch.testing.assert_close(v4.forward_routed(x, weights, ids, ad, plan).float(), v4.forward_routed(x, weights, ids).float(), rtol=2 ** -6, atol=2 ** -6)
+    none = AdapterPlan(torch.zeros(0, dtype=torch.int32, device=DEV), 1)
+    for each in (layer, v4):
+        assert each(x[:0], logits[:0], adapters=ad, plan=none).shape == (0, H)
 
 
 @gpu
-def test_captured_steps_follow_their_inputs():
+@pytest.mark.parametrize("T,r", [(48, 16), (1000, 16), (3000, 64)])
+def test_captured_steps_follow_their_inputs(T, r):
     """Router, plan and adapters in one captured graph: replayed on other logits, rows and requests, another adapter loaded."""
-    E, n, K, N, T = 64, 4, 256, 128, 48
-    A, B, scale, ad = make(n, K, N, 16, BF16, 2)
+    E, n, K, N = 64, 4, 256, 128
+    A, B, scale, ad = make(n, K, N, r, BF16, 2)
     g = gen(12)
     x, base = torch.randn(T, K, generator=g, device=DEV).to(BF16), torch.randn(T, N, generator=g, device=DEV)
     logits = torch.randn(T, E, generator=g, device=DEV)
-    offsets = torch.tensor([0, 10, 30, 48], dtype=torch.int32, device=DEV)
+    offsets = torch.tensor([0, 10, 30, T], dtype=torch.int32, device=DEV)
     slots = torch.tensor([0, 2, -1], dtype=torch.int32, device=DEV)
 
     def step():
@@ -727,7 +870,7 @@ def test_captured_steps_follow_their_inputs():
     for turn in range(3):
         x.copy_(torch.randn(T, K, generator=g, device=DEV).to(BF16))
         logits.copy_(torch.randn(T, E, generator=g, device=DEV))
-        offsets.copy_(torch.tensor([[0, 1, 2, 48], [0, 0, 48, 48], [0, 5, 9, 20]][turn], dtype=torch.int32))
+        offsets.copy_(torch.tensor([[0, 1, 2, T], [0, 0, T, T], [0, 5, 9, 20]][turn], dtype=torch.int32))
         slots.copy_(torch.tensor([[3, 1, 0], [1, 1, 1], [2, 7, 0]][turn], dtype=torch.int32))
         ad.load(1, A[turn], B[turn], 0.5 + turn)
         graph.replay()
@@ -736,12 +879,13 @@ def test_captured_steps_follow_their_inputs():
 
 
 @gpu
-def test_two_streams_at_once():
-    A, B, scale, ad = make(4, 1024, 512, 32, BF16, 2)
+@pytest.mark.parametrize("rows,r", [(300, 32), (1000, 32), (3000, 64)])
+def test_two_streams_at_once(rows, r):
+    A, B, scale, ad = make(4, 1024, 512, r, BF16, 2)
     g = gen(13)
-    xs = [torch.randn(300, 1024, generator=g, device=DEV).to(BF16) for _ in range(2)]
-    bases = [torch.randn(300, 512, generator=g, device=DEV) for _ in range(2)]
-    plans = [AdapterPlan(torch.randint(-1, 4, (300,), generator=g, device=DEV), 4) for _ in range(2)]
+    xs = [torch.randn(rows, 1024, generator=g, device=DEV).to(BF16) for _ in range(2)]
+    bases = [torch.randn(rows, 512, generator=g, device=DEV) for _ in range(2)]
+    plans = [AdapterPlan(torch.randint(-1, 4, (rows,), generator=g, device=DEV), 4) for _ in range(2)]
     want = [ad(x, p, base=b) for x, p, b in zip(xs, plans, bases)]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
