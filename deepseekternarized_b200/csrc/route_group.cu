@@ -8,10 +8,10 @@
 //   weight_i = s of pick i, divided by the picks' sum + 1e-20 when renormalised (top_k > 1), times route_scale
 //
 // The picks are those of exact arithmetic. Without a bias f keeps the order of the logits, which decide by themselves; sums of two
-// scores and keys with a bias are compared in float32 where they are further apart than their rounding errors can reach. Picks that
-// are closer are told apart in 64 bits by themselves, where that takes no sum over all experts; a token with closer groups is done
-// again in 64 bits by its block. A NaN ranks above every number (such a token goes that way too), so a token's ids are distinct and
-// inside [0, E) whatever the logits hold. A token done again costs its block 4 to 7 us (256 experts), a few close picks 1.
+// scores and keys with a bias are compared in float32 where they are further apart than their rounding errors can reach. Groups and
+// picks that are closer are told apart in 64 bits by themselves; where that takes a sum over all experts (softmax with a bias) or
+// there are many of them, the token is done again in 64 bits by its block, which costs that 4 to 7 us (256 experts). A NaN ranks
+// above every number (such a token goes that way too), so a token's ids are distinct and inside [0, E) whatever the logits hold.
 #include "dst_common.cuh"
 
 namespace dst {
@@ -247,10 +247,10 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
     }
   }
   // The lane's numbers in blocks of eight. A logit is negated under a negative temperature: experts rank by it as they do by their
-  // scores. zmax, zmin and `special` (a NaN from anything that is not finite) come out of the first pass.
+  // scores. On the way: the largest magnitude, softmax's largest, and `special`, a NaN from anything that is not finite.
   const bool flip = a.temp < 0.f;
   const float inv_temp = 1.f / fabsf(a.temp);
-  float zmax = -INFINITY, zmin = INFINITY, special = 0.f, inv_sum = 1.f, mx = 0.f;
+  float zmax = -INFINITY, zabs = 0.f, special = 0.f, inv_sum = 1.f, mx = 0.f;
   const auto eight = [&](int j0, float (&z)[8]) {
     const float4 u = *reinterpret_cast<const float4*>(own + j0), v = *reinterpret_cast<const float4*>(own + j0 + 4);
     z[0] = u.x, z[1] = u.y, z[2] = u.z, z[3] = u.w, z[4] = v.x, z[5] = v.y, z[6] = v.z, z[7] = v.w;
@@ -264,19 +264,19 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
       for (int i = 0; i < 8; ++i) z[i] = -z[i];
     }
   };
-  const auto range = [&](const float (&z)[8]) {
+  const auto range = [&](const float (&z)[8], bool numbers) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      zmax = fmaxf(zmax, z[i]);
-      zmin = fminf(zmin, z[i]);
-      special = fmaf(z[i], 0.f, special);
+      if (SCORE == DST_SCORE_SOFTMAX) zmax = fmaxf(zmax, z[i]);
+      zabs = fmaxf(zabs, fabsf(z[i]));
+      if (numbers) special = fmaf(z[i], 0.f, special);
     }
   };
   if (SCORE == DST_SCORE_SOFTMAX) {
     for (int j0 = 0; j0 < n; j0 += 8) {
       float z[8];
       eight(j0, z);
-      range(z);
+      range(z, true);
     }
     mx = value_of(seg_max(order_of(zmax))) * inv_temp;
     float sum = 0.f;
@@ -297,8 +297,8 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
   for (int j0 = 0; j0 < n; j0 += 8) {
     float z[8];
     eight(j0, z);
-    if (SCORE != DST_SCORE_SOFTMAX) range(z);
-    if (a.bias) {
+    if (SCORE != DST_SCORE_SOFTMAX) range(z, !a.bias);
+    if (a.bias) {  // a NaN shows in the key, an infinity in zabs
       float b[8];
       if (a.vec_bias) {
         const float4 u = __ldg(reinterpret_cast<const float4*>(a.bias + id0 + j0)), v = __ldg(reinterpret_cast<const float4*>(a.bias + id0 + j0 + 4));
@@ -332,28 +332,34 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
     }
   }
   bool again = false;
-  if (__any_sync(FULL, special != 0.f || special_key != 0.f)) {  // NaNs, infinities above and NaN keys: in 64 bits
-    zmin = INFINITY;
+  if (__any_sync(FULL, special != 0.f || special_key != 0.f || zabs == INFINITY)) {  // NaNs, infinities above and NaN keys: in 64 bits
+    zabs = 0.f;
     for (int j = 0; j < n; ++j) {
       const float v = load_logit(a, row + id0 + j), z = flip ? -v : v, b = a.bias ? a.bias[id0 + j] : 0.f;
       again = again || !(z < INFINITY) || b != b;
-      zmin = fminf(zmin, z == -INFINITY ? INFINITY : z);
+      zabs = fmaxf(zabs, z == -INFINITY ? 0.f : fabsf(z));
     }
     again = seg_any(again);
   }
-  zmax = value_of(seg_max(order_of(zmax)));
-  again = again || (SCORE == DST_SCORE_SOFTMAX && zmax == -INFINITY);  // nothing to divide by
+  if (SCORE == DST_SCORE_SOFTMAX) {
+    zmax = value_of(seg_max(order_of(zmax)));
+    again = again || zmax == -INFINITY;  // nothing to divide by
+  }
   // the error of a near score in units of 2^-24 of the largest one: 20 of its own steps, 2 |z| of the exponential's argument (4 |z|
   // for softmax's difference, whose sum adds one per expert of a lane and a few), 6 |z| where a temperature rounds z; a key's own
   // rounding comes on top where it is used
   float delta = 0.f;
   if (a.bias || a.two) {
-    const float largest = SCORE == DST_SCORE_SOFTMAX ? inv_sum : SCORE == DST_SCORE_SIGMOID ? 1.f : sqrtf(fmaxf(zmax * inv_temp, 0.f) + 0.7f);
+    const float far = __uint_as_float(seg_max(__float_as_uint(zabs))) * inv_temp;  // of the finite ones
+    const float largest = SCORE == DST_SCORE_SOFTMAX ? inv_sum : SCORE == DST_SCORE_SIGMOID ? 1.f : sqrtf(far + 0.7f);
     const float per_z = (SCORE == DST_SCORE_SOFTMAX ? 4.f : 2.f) + (inv_temp == 1.f ? 0.f : 6.f);
-    const float low = value_of(~seg_max(~order_of(zmin)));  // the smallest finite one; an infinity where there is none
-    const float far = fmaxf(fabsf(zmax) < INFINITY ? fabsf(zmax) : 0.f, low < INFINITY ? fabsf(low) : 0.f) * inv_temp;
     delta = largest * (20.f + (SCORE == DST_SCORE_SOFTMAX ? a.chunk + 8.f : 0.f) + per_z * far) * 0x1p-24f;
   }
+
+  const auto key64 = [&](float z, float b) {  // softmax: without the division by the sum of all, for comparisons without a bias
+    const double v = a.temp == 1.f ? (double)z : (double)z / (double)a.temp;
+    return score64<SCORE>(v, SCORE == DST_SCORE_SOFTMAX ? (double)zmax / fabs((double)a.temp) : 0.0, 1.0) + (double)b;
+  };
 
   // groups
   if (a.kept < a.groups) {
@@ -371,7 +377,7 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
       const uint32_t o = __shfl_sync(FULL, g, h << a.shift, LPT);
       better += o > g || (o == g && h < group);
     }
-    const bool keep = in && better < a.kept;
+    bool keep = in && better < a.kept;
     if (sums || a.bias) {  // how near the border is
       const uint32_t last = ~seg_max(keep ? ~g : 0u), next = seg_max(in && !keep ? g : 0u);
       const float l = value_of(last), x = value_of(next), tol = (sums ? 4.f : 2.f) * delta + 0x1p-22f * fabsf(l);
@@ -381,8 +387,51 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
         const bool close = border && in && fabsf(value_of(g) - l) <= tol;
         const int ref = __ffs(__ballot_sync(FULL, close) & segment) - 1;
         const uint32_t r1 = __shfl_sync(FULL, m1, max(ref, 0)), r2 = __shfl_sync(FULL, m2, max(ref, 0));
-        const bool other = seg_any(close && (m1 != r1 || m2 != r2));
-        again = again || (border && (a.bias || ref < 0 || other));
+        const bool other = seg_any(close && (m1 != r1 || m2 != r2)), unsure = border && (a.bias || ref < 0 || other);
+        again = again || (unsure && (ref < 0 || (SCORE == DST_SCORE_SOFTMAX && a.bias)));
+        const bool look = unsure && !again;
+        if (__any_sync(FULL, look)) {
+          // The close groups in 64 bits; they share the places that those among them had. A lane looks at its two largest keys; a
+          // third that may be among its group's largest: the other form.
+          double v1 = -INFINITY, v2 = -INFINITY;
+          bool lost = false;
+          if (look && close) {
+            if (!a.bias) {  // by the logits, which are exact
+              const float z1 = value_of(m1), z2 = value_of(m2);
+              v1 = key64(flip ? -z1 : z1, 0.f), v2 = key64(flip ? -z2 : z2, 0.f);
+            } else {
+              const float least = value_of(sums ? m2 : m1), reach = 2.f * delta + 0x1p-22f * fabsf(least);
+              const auto may = [&](uint32_t k) { return k && !(least - value_of(k) > reach); };
+              lost = may(top[2]);
+              bool first = may(top[0]), second = may(top[1]);
+              for (int j = 0; j < n && (first || second); ++j) {
+                const bool is_first = first && own[j] == top[0];
+                if (is_first || (second && own[j] == top[1])) {
+                  const double k = key64(load_logit(a, row + id0 + j), a.bias[id0 + j]);
+                  v2 = fmax(v2, fmin(v1, k)), v1 = fmax(v1, k);
+                  (is_first ? first : second) = false;
+                }
+              }
+            }
+          }
+          if (a.bias) {
+            for (int off = 1; off < (1 << a.shift); off <<= 1) {
+              const double o1 = __shfl_xor_sync(FULL, v1, off), o2 = __shfl_xor_sync(FULL, v2, off);
+              v2 = fmax(fmin(v1, o1), fmax(v2, o2)), v1 = fmax(v1, o1);
+            }
+          }
+          const uint64_t exact = order_of(sums ? v1 + v2 : v1);
+          int rank = 0, places = 0;
+          for (int h = 0; h < a.groups; ++h) {
+            const uint64_t o = __shfl_sync(FULL, exact, h << a.shift, LPT);
+            const int kind = __shfl_sync(FULL, (close ? 2 : 0) | (keep ? 1 : 0), h << a.shift, LPT);
+            places += kind == 3;
+            rank += kind >= 2 && (o > exact || (o == exact && h < group));
+          }
+          const bool any_lost = seg_any(lost);
+          again = again || any_lost;
+          if (look && close) keep = rank < places;
+        }
       }
     }
     if (!keep) {
@@ -475,11 +524,8 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
           if (own[j] == top[0] && skip-- == 0) next = j;
       const int extra_id = id0 + next;
       const float extra_z = extra ? load_logit(a, row + extra_id) : 0.f;
-      const auto key64 = [&](float z, int e) {
-        const double v = a.temp == 1.f ? (double)z : (double)z / (double)a.temp;
-        return order_of(score64<SCORE>(v, 0.0, 1.0) + (double)a.bias[e]);
-      };
-      const uint64_t own_key = pick ? key64(flip ? -zi : zi, id) : 0, extra_key = extra ? key64(extra_z, extra_id) : 0;
+      const uint64_t own_key = pick ? order_of(key64(flip ? -zi : zi, b)) : 0;
+      const uint64_t extra_key = extra ? order_of(key64(extra_z, a.bias[extra_id])) : 0;
       int own_rank = 0, extra_rank = 0;
       const auto against = [&](uint64_t key, int e) {
         own_rank += key > own_key || (key == own_key && e < id);

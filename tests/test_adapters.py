@@ -39,27 +39,19 @@ def route64(logits, k, scale, renorm, score, bias, temp, groups, kept, group_sco
     s = {"softmax": lambda: torch.softmax(v, -1), "sigmoid": lambda: torch.sigmoid(v),
          "sqrtsoftplus": lambda: torch.logaddexp(v, torch.zeros_like(v)).sqrt()}[score]()
     key = s if bias is None else s + bias.double().cpu()
-    w, ids = np.empty((T, k)), np.empty((T, k), np.int64)
     size = E // groups
 
-    def first(values):  # positions in descending order: NaN, then numbers; stable
-        return sorted(range(len(values)), key=lambda i: (0, 0.0) if np.isnan(values[i]) else (1, -values[i]))
+    def first(values):  # positions in descending order
+        return values.sort(dim=-1, descending=True, stable=True).indices
 
-    for t in range(T):
-        row = key[t].numpy()
-        g = []
-        for i in range(groups):
-            part = row[i * size:(i + 1) * size]
-            best = [part[j] for j in first(part)[:2 if group_score == "top2" else 1]]
-            g.append(np.nan if np.isnan(sum(best)) else float(sum(best)))
-        allowed = sorted(first(g)[:kept])
-        cand = [i * size + j for i in allowed for j in range(size)]
-        pick = [cand[j] for j in first(row[cand])[:k]]
-        ids[t] = pick
-        w[t] = s[t].numpy()[pick]
-        if renorm and k > 1:
-            w[t] /= w[t].sum() + 1e-20
-    return w * scale, ids
+    best = key.view(T, groups, size).sort(dim=-1, descending=True).values[..., :2 if group_score == "top2" else 1].sum(-1)
+    allowed = first(best)[:, :kept].sort(dim=-1).values
+    cand = (allowed[..., None] * size + torch.arange(size)).flatten(1)
+    ids = cand.gather(1, first(key.gather(1, cand))[:, :k])
+    w = s.gather(1, ids)
+    if renorm and k > 1:
+        w = w / (w.sum(-1, keepdim=True) + 1e-20)
+    return (w * scale).numpy(), ids.numpy()
 
 
 def check_route(logits, k, scale=1.0, renorm=True, score="sigmoid", bias=None, temp=1.0, groups=8, kept=4, group_score="top2"):
@@ -152,6 +144,32 @@ def test_route_groups_near_picks(T, E, groups, kept, k, score):
     bias[::5] = 2.0 ** -26
     check_route(logits, k, 1.0, True, score, bias, 1.0, groups, kept, "max")
     check_route(-1.5 * logits, k, 1.0, False, score, bias, -1.5, groups, kept, "max")
+
+
+@gpu
+@pytest.mark.parametrize("T,E,groups,kept,k", [(5000, 256, 8, 4, 8), (5000, 384, 6, 1, 6), (3000, 256, 8, 7, 3), (9, 256, 8, 4, 8), (11, 128, 4, 2, 4),
+                                               (2500, 320, 10, 3, 5), (9, 1024, 4, 2, 8)])
+@pytest.mark.parametrize("score,group_score,with_bias", [("sigmoid", "top2", True), ("sqrtsoftplus", "top2", False), ("softmax", "top2", False),
+                                                         ("sqrtsoftplus", "max", True), ("softmax", "max", True)])
+def test_route_groups_near_groups(T, E, groups, kept, k, score, group_score, with_bias):
+    """Groups whose scores differ by less than their rounding at the border, up to all of them: two high experts each, or three
+    (several largest ones to choose from), on lanes of their own or on one."""
+    g = gen(E + kept)
+    size = E // groups
+    logits = torch.rand(T, groups, size, generator=g, device=DEV) - 4.0
+    steps = torch.randint(0, 4, (T, groups, 3), generator=g, device=DEV).to(torch.int32)
+    high = (torch.tensor([2.0, 1.25, 1.25], device=DEV).view(torch.int32) + steps).view(torch.float32)
+    at = torch.rand(T, groups, size, generator=g, device=DEV).argsort(dim=-1)[..., :3]
+    third = torch.rand(T, groups, generator=g, device=DEV) < 0.1
+    high[..., 2] = torch.where(third, high[..., 2], -3.0)
+    far = torch.rand(T, groups, generator=g, device=DEV) < torch.rand(T, 1, generator=g, device=DEV)
+    high += torch.where(far, torch.rand(T, groups, generator=g, device=DEV) - 0.5, 0.0)[..., None]
+    logits = logits.scatter(-1, at, high).view(T, E).contiguous()
+    bias = torch.zeros(E, device=DEV) if with_bias else None
+    if with_bias:
+        bias[::7] = 2.0 ** -25
+    check_route(logits, k, 1.0, True, score, bias, 1.0, groups, kept, group_score)
+    check_route(-1.5 * logits, k, 1.0, False, score, bias, -1.5, groups, kept, group_score)
 
 
 @gpu
