@@ -920,72 +920,74 @@ __global__ void __launch_bounds__(256, RP <= 64 ? 2 : 1) adapter_columns_kernel(
   if (c.kind == 1) return run(Int<BASE_F32>(), Int<1>());
   if (c.kind == 2) return run(Int<BASE_T>(), Int<0>());
   if (c.kind == 3) return run(Int<BASE_NONE>(), Int<0>());
-  if constexpr (!SHARED) {
-    // Any types and alignment: the sums go through shared memory, so that a warp reads and writes 32 neighbouring columns of a row at
-    // a time; base is read a step ahead.
-    using NP = Int<BF ? 3 : 2>;
-    const int64_t oa = row_at(g), ob = row_at(g + 8);
-    float next[16];
-    const auto base_of = [&](int step) {
-      const int64_t col = column(step) + lane;
-      const bool in = step < steps && col < (P == 2 && step < per_part ? Np : N);
+  // Any types and alignment: the sums go through shared memory, so that a warp reads and writes 32 neighbouring columns of a row at
+  // a time; base is read a step ahead.
+  using NP = Int<BF ? 3 : 2>;
+  constexpr int AHEAD = SHARED ? BS - 1 : BS;
+  const int64_t oa = row_at(g), ob = row_at(g + 8);
+  float next[16];
+  const auto base_of = [&](int step) {
+    const int64_t col = column(step) + lane;
+    const bool in = step < steps && col < (P == 2 && step < per_part ? Np : N);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t row = __shfl_sync(0xffffffffu, r < 8 ? oa : ob, (r & 7) * 4);
-        next[r] = in && c.base && r < rows ? element(c.base, row * c.base_stride + col, c.base_dtype) : 0.f;
-      }
-    };
-#pragma unroll
-    for (int s = 0; s < BS; ++s) {
-      const int step = worker + s * workers;
-      if (step < steps) fetch_b(b + (int64_t)column(step) * RP, s);
-      commit();
+    for (int r = 0; r < 16; ++r) {
+      const int64_t row = __shfl_sync(0xffffffffu, r < 8 ? oa : ob, (r & 7) * 4);
+      next[r] = in && c.base && r < rows ? element(c.base, row * c.base_stride + col, c.base_dtype) : 0.f;
     }
-    base_of(worker);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    int part = P == 2 && worker >= per_part, stage = 0;
-    load_h(NP(), part);
-    for (int step = worker; step < steps; step += workers) {
-      if (P == 2 && part == 0 && step >= per_part) part = 1, load_h(NP(), part);
-      wait_but<BS - 1>();
-      float d[4][4], mine[16];
-      zero(d);
-      product(NP(), stage, d);
+  };
+  const auto fetch = [&](int step, int stage) {
+    if (step < steps) fetch_b(b + (int64_t)column(step) * RP, stage);
+    commit();
+  };
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mine[r] = next[r];
-      base_of(step + workers);
-      const uint32_t at = part0 + stage * S::BST;
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float f = factor[half];
-          asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(at + (g + 8 * half) * 128 + (eight ? 8 * q + 4 * u : 16 * u + 4 * q) * 4),
-                       "f"(d[2 * u][2 * half] * f), "f"(d[2 * u][2 * half + 1] * f), "f"(d[2 * u + 1][2 * half] * f),
-                       "f"(d[2 * u + 1][2 * half + 1] * f)
-                       : "memory");
-        }
-      __syncwarp();
-      const int64_t col = column(step) + lane;
-      const bool in = col < (P == 2 && step < per_part ? Np : N);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t row = __shfl_sync(0xffffffffu, r < 8 ? oa : ob, (r & 7) * 4);
-        float v;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at + r * 128 + lane * 4) : "memory");
-        v += mine[r];
-        if (in && r < rows) {
-          const int64_t o = row * c.out_stride + col;
-          if (c.out_dtype == DST_OUT_F32) static_cast<float*>(c.out)[o] = v;
-          else if (c.out_dtype == DST_OUT_BF16) static_cast<__nv_bfloat16*>(c.out)[o] = __float2bfloat16_rn(v);
-          else static_cast<__half*>(c.out)[o] = __float2half_rn(v);
-        }
-      }
-      __syncwarp();
-      if (step + BS * workers < steps) fetch_b(b + (int64_t)column(step + BS * workers) * RP, stage);
-      commit();
-      stage = stage + 1 == BS ? 0 : stage + 1;
+  for (int s = 0; s < AHEAD; ++s) fetch(worker + s * workers, s);
+  base_of(worker);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int part = P == 2 && worker >= per_part, stage = 0;
+  load_h(NP(), part);
+  for (int step = worker; step < steps; step += workers) {
+    if (P == 2 && part == 0 && step >= per_part) part = 1, load_h(NP(), part);
+    wait_but<AHEAD - 1>();
+    if (SHARED) {  // one barrier a step, as above
+      __syncthreads();
+      fetch(step + AHEAD * workers, stage == 0 ? BS - 1 : stage - 1);
     }
+    float d[4][4], mine[16];
+    zero(d);
+    product(NP(), stage, d);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mine[r] = next[r];
+    base_of(step + workers);
+    const uint32_t at = part0 + stage * S::BST;
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float f = factor[half];
+        asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(at + (g + 8 * half) * 128 + (eight ? 8 * q + 4 * u : 16 * u + 4 * q) * 4),
+                     "f"(d[2 * u][2 * half] * f), "f"(d[2 * u][2 * half + 1] * f), "f"(d[2 * u + 1][2 * half] * f),
+                     "f"(d[2 * u + 1][2 * half + 1] * f)
+                     : "memory");
+      }
+    __syncwarp();
+    const int64_t col = column(step) + lane;
+    const bool in = col < (P == 2 && step < per_part ? Np : N);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int64_t row = __shfl_sync(0xffffffffu, r < 8 ? oa : ob, (r & 7) * 4);
+      float v;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at + r * 128 + lane * 4) : "memory");
+      v += mine[r];
+      if (in && r < rows) {
+        const int64_t o = row * c.out_stride + col;
+        if (c.out_dtype == DST_OUT_F32) static_cast<float*>(c.out)[o] = v;
+        else if (c.out_dtype == DST_OUT_BF16) static_cast<__nv_bfloat16*>(c.out)[o] = __float2bfloat16_rn(v);
+        else static_cast<__half*>(c.out)[o] = __float2half_rn(v);
+      }
+    }
+    __syncwarp();
+    if (!SHARED) fetch(step + BS * workers, stage);
+    stage = stage + 1 == BS ? 0 : stage + 1;
   }
 }
 
@@ -1004,12 +1006,12 @@ int launch_cluster(const AdapterCall& c, int64_t max_tiles, cudaStream_t st) {
   return DST_OK;
 }
 
-template <typename T, int RP, int P, bool SHARED>
+template <typename T, int RP, int P, bool SHARED_A, bool SHARED_B>
 int launch_two(AdapterCall c, int64_t max_tiles, cudaStream_t st) {
-  using H = HShape<RP * P, SHARED>;
-  using C = CShape<RP, SHARED>;
-  auto h_kernel = adapter_h_kernel<T, RP * P, SHARED>;
-  auto c_kernel = adapter_columns_kernel<T, RP, P, SHARED>;
+  using H = HShape<RP * P, SHARED_A>;
+  using C = CShape<RP, SHARED_B>;
+  auto h_kernel = adapter_h_kernel<T, RP * P, SHARED_A>;
+  auto c_kernel = adapter_columns_kernel<T, RP, P, SHARED_B>;
   DST_CUDA_TRY(cudaFuncSetAttribute(h_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, H::SMEM));
   DST_CUDA_TRY(cudaFuncSetAttribute(c_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
   const int columns = c.splits;
@@ -1031,9 +1033,10 @@ template <typename T, int RP, int P>
 int launch(const AdapterCall& c, int64_t max_tiles, cudaStream_t st) {
   if (c.ctas) return launch_cluster<T, RP, P>(c, max_tiles, st);
   if constexpr (RP >= 64) {
-    if (c.shared) return launch_two<T, RP, P, true>(c, max_tiles, st);
+    if (c.shared_a) return launch_two<T, RP, P, true, true>(c, max_tiles, st);
+    if (c.shared_b) return launch_two<T, RP, P, false, true>(c, max_tiles, st);
   }
-  return launch_two<T, RP, P, false>(c, max_tiles, st);
+  return launch_two<T, RP, P, false, false>(c, max_tiles, st);
 }
 
 template <typename T>
