@@ -7,13 +7,13 @@ namespace dst {
 namespace {
 
 // How a call is cut: CTAs of a cluster (0: two kernels); warps of 16 rows for h inside a CTA and CTAs of them; those for the columns;
-// whether the row blocks of a tile share A (rows of x that are aligned) and B
+// whether the row blocks of a tile share A and B
 struct Cut {
-  int ctas, share, k_splits, columns, shared_a, shared_b;
+  int ctas, share, k_splits, columns, shared;
 };
-Cut cut_of(int64_t max_tiles, int tile, int64_t K_padded, int64_t N, int rank_padded, bool x_vec) {
+Cut cut_of(int64_t max_tiles, int tile, int64_t K_padded, int64_t N, int rank_padded) {
   const int64_t sms = sm_count(), blocks = max_tiles * (tile / 16);
-  Cut cut{0, 8, 1, 1, 0, 0};
+  Cut cut{0, 8, 1, 1, 0};
   // Up to 48 blocks the cluster's one launch costs the host 5 us less (11 against 16 a call) and the device as much: 1 row of 4096 x
   // 4096 4.2 us against 4.1, 333 rows 8.0 against 8.2, 48 pairs (rank 16 twice) 13.1 against 14.4 with their plan; 64 rows of 37
   // adapters (53 blocks) through 11008 x 4096 14.9 against 11.2. A cluster takes tiles of 16 rows only.
@@ -40,10 +40,10 @@ Cut cut_of(int64_t max_tiles, int tile, int64_t K_padded, int64_t N, int rank_pa
     }
     return n;
   };
-  cut.shared_b = tile == 128 && rank_padded >= 64, cut.shared_a = cut.shared_b && x_vec;
+  cut.shared = tile == 128 && rank_padded >= 64;
   const int h = warps(K_padded / 64, rank_padded >= 64 ? 2 : 1, 4, 12, 22, 4);
   cut.columns = warps((N + 31) / 32, 1, 8, 16, 32, 5);
-  cut.share = cut.shared_a ? 1 : std::min(h, 8), cut.k_splits = std::min(cut.shared_a ? h : std::max(h / 8, 1), 16);
+  cut.share = cut.shared ? 1 : std::min(h, 8), cut.k_splits = std::min(cut.shared ? h : std::max(h / 8, 1), 16);
   return cut;
 }
 
@@ -58,10 +58,8 @@ extern "C" size_t dst_adapter_workspace_bytes(const dst_adapters* w, const dst_a
   using namespace dst;
   if (!w || !plan || plan->max_tiles <= 0 || plan->positions <= 0 || w->parts < 1 || w->rank_padded < 1 || w->K_padded < 1 || w->N < 1)
     return 0;
-  // for either form of h: which one it is depends on the alignment of x too
-  const Cut one = cut_of(plan->max_tiles, plan->tile, w->K_padded, w->N, w->rank_padded, true);
-  const Cut two = cut_of(plan->max_tiles, plan->tile, w->K_padded, w->N, w->rank_padded, false);
-  return one.ctas ? 0 : (size_t)std::max(one.k_splits, two.k_splits) * plan->positions * w->parts * w->rank_padded * sizeof(float);
+  const Cut cut = cut_of(plan->max_tiles, plan->tile, w->K_padded, w->N, w->rank_padded);
+  return cut.ctas ? 0 : (size_t)cut.k_splits * plan->positions * w->parts * w->rank_padded * sizeof(float);
 }
 
 extern "C" int dst_adapter_apply(const dst_adapters* w, const dst_adapter_rows* plan, const void* x, int64_t x_stride, const void* base,
@@ -96,8 +94,8 @@ extern "C" int dst_adapter_apply(const dst_adapters* w, const dst_adapter_rows* 
     if (base && base_dtype == DST_OUT_F32 && (out_dtype == own || out_dtype == DST_OUT_F32)) c.kind = out_dtype == own ? 0 : 1;
     else if (out_dtype == own && (!base || base_dtype == own)) c.kind = base ? 2 : 3;
   }
-  const Cut cut = cut_of(plan->max_tiles, plan->tile, w->K_padded, w->N, w->rank_padded, c.x_vec);
-  c.sub = plan->tile / 16, c.shared_a = cut.shared_a, c.shared_b = cut.shared_b, c.ctas = cut.ctas, c.share = cut.share, c.k_splits = cut.k_splits, c.splits = cut.columns;
+  const Cut cut = cut_of(plan->max_tiles, plan->tile, w->K_padded, w->N, w->rank_padded);
+  c.sub = plan->tile / 16, c.shared = cut.shared, c.ctas = cut.ctas, c.share = cut.share, c.k_splits = cut.k_splits, c.splits = cut.columns;
   c.positions = plan->positions, c.h = static_cast<float*>(workspace);
   if (!cut.ctas) {
     if (!workspace || workspace_bytes < dst_adapter_workspace_bytes(w, plan)) return DST_ERR_BAD_ARG;

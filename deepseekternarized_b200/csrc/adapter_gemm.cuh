@@ -508,8 +508,9 @@ __global__ void __launch_bounds__(256, 2) adapter_h_kernel(const AdapterCall c) 
       mma16(acc[i], u.z, v.z, u.w, v.w, w.z, w.w, T());
     }
   };
+  constexpr int AHEAD = SHARED ? XS - 1 : XS;  // SHARED: one barrier a step; behind it every warp is done with the step before, whose slots are filled again
   if (n == 0) {
-  } else if (SHARED || c.x_vec) {
+  } else if (c.x_vec) {
     // eight lanes a row, 128 bytes of it; a lane multiplies the pieces q and q + 4 of its two rows. Every other row's halves are
     // swapped, so that eight lanes find their pieces in different banks.
     const char* at[4];
@@ -536,8 +537,6 @@ __global__ void __launch_bounds__(256, 2) adapter_h_kernel(const AdapterCall c) 
       }
       commit();
     };
-    // SHARED: one barrier a step. Behind it every warp is done with the step before, whose slots are filled again.
-    constexpr int AHEAD = SHARED ? XS - 1 : XS;
 #pragma unroll
     for (int s = 0; s < AHEAD; ++s) fetch(s, s);
     for (int i = 0; i < n; i += XS) {
@@ -609,17 +608,24 @@ __global__ void __launch_bounds__(256, 2) adapter_h_kernel(const AdapterCall c) 
                         __funnelshift_r(w[3], w[4], bits));
     };
 #pragma unroll
-    for (int s = 0; s < XS; ++s) fetch(s, s);
+    for (int s = 0; s < AHEAD; ++s) fetch(s, s);
     for (int i = 0; i < n; i += XS) {
 #pragma unroll
       for (int s = 0; s < XS; ++s) {
         if (i + s < n) {
-          wait_but<XS - 1>();
-          __syncwarp();  // the pieces of all lanes
+          wait_but<AHEAD - 1>();
+          if (SHARED) {
+            __syncthreads();
+            fetch(i + s + AHEAD, (s + AHEAD) % XS);
+          } else {
+            __syncwarp();  // the pieces of all lanes
+          }
           multiply(s, 0, shifted(from_a + s * S::XST, ma), shifted(from_b + s * S::XST, mb));
           multiply(s, 1, shifted(from_a + s * S::XST + 64, ma), shifted(from_b + s * S::XST + 64, mb));
-          __syncwarp();  // taken by all
-          fetch(i + s + XS, s);
+          if (!SHARED) {
+            __syncwarp();  // taken by all
+            fetch(i + s + XS, s);
+          }
         }
       }
     }
@@ -659,7 +665,8 @@ __global__ void __launch_bounds__(256, 2) adapter_h_kernel(const AdapterCall c) 
 template <int RP, bool SHARED>
 struct CShape {
   static constexpr int BB = RP == 16 ? 1024 : RP / 32 * 2048, BASE = 2048, BST = BASE + (SHARED ? 0 : BB);  // bytes of a step: base, B
-  static constexpr int BS = SHARED || RP == 16 ? 4 : RP == 32 ? 3 : 2, BPART = BS * BST, SMEM = 8 * BPART + (SHARED ? BS * BB : 0);
+  static constexpr int BS = SHARED || RP == 16 ? 4 : RP == 32 ? 3 : 2, BPART = BS * BST;
+  static constexpr int PLACES = 8 * BPART + (SHARED ? BS * BB : 0), SMEM = PLACES + 8 * 256;  // where a warp's 16 rows of base and result are
 };
 
 template <typename T, int RP, int P, bool SHARED>
@@ -924,16 +931,32 @@ __global__ void __launch_bounds__(256, RP <= 64 ? 2 : 1) adapter_columns_kernel(
   // a time; base is read a step ahead.
   using NP = Int<BF ? 3 : 2>;
   constexpr int AHEAD = SHARED ? BS - 1 : BS;
-  const int64_t oa = row_at(g), ob = row_at(g + 8);
+  char** places = reinterpret_cast<char**>(smem + S::PLACES + warp * 256);  // of the rows of base, then of the result
+  if (lane < 16) {
+    places[lane] = const_cast<char*>(static_cast<const char*>(c.base)) + row_at(lane) * c.base_stride * (c.base_dtype == DST_OUT_F32 ? 4 : 2);
+    places[lane + 16] = static_cast<char*>(c.out) + row_at(lane) * c.out_stride * (c.out_dtype == DST_OUT_F32 ? 4 : 2);
+  }
+  __syncwarp();
   float next[16];
   const auto base_of = [&](int step) {
     const int64_t col = column(step) + lane;
-    const bool in = step < steps && col < (P == 2 && step < per_part ? Np : N);
+    const bool in = c.base && step < steps && col < (P == 2 && step < per_part ? Np : N);
+    const auto read = [&](auto type) {
+      using V = decltype(type);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int64_t row = __shfl_sync(0xffffffffu, r < 8 ? oa : ob, (r & 7) * 4);
-      next[r] = in && c.base && r < rows ? element(c.base, row * c.base_stride + col, c.base_dtype) : 0.f;
-    }
+      for (int r = 0; r < 16; ++r) {
+        next[r] = 0.f;
+        if (in && r < rows) {
+          const V v = reinterpret_cast<const V*>(places[r])[col];
+          if constexpr (std::is_same<V, float>::value) next[r] = v;
+          else if constexpr (std::is_same<V, __half>::value) next[r] = __half2float(v);
+          else next[r] = __bfloat162float(v);
+        }
+      }
+    };
+    if (c.base_dtype == DST_OUT_F32) read(float());
+    else if (c.base_dtype == DST_OUT_BF16) read(__nv_bfloat16());
+    else read(__half());
   };
   const auto fetch = [&](int step, int stage) {
     if (step < steps) fetch_b(b + (int64_t)column(step) * RP, stage);
@@ -972,19 +995,24 @@ __global__ void __launch_bounds__(256, RP <= 64 ? 2 : 1) adapter_columns_kernel(
     __syncwarp();
     const int64_t col = column(step) + lane;
     const bool in = col < (P == 2 && step < per_part ? Np : N);
+    const auto write = [&](auto type) {
+      using V = decltype(type);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int64_t row = __shfl_sync(0xffffffffu, r < 8 ? oa : ob, (r & 7) * 4);
-      float v;
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at + r * 128 + lane * 4) : "memory");
-      v += mine[r];
-      if (in && r < rows) {
-        const int64_t o = row * c.out_stride + col;
-        if (c.out_dtype == DST_OUT_F32) static_cast<float*>(c.out)[o] = v;
-        else if (c.out_dtype == DST_OUT_BF16) static_cast<__nv_bfloat16*>(c.out)[o] = __float2bfloat16_rn(v);
-        else static_cast<__half*>(c.out)[o] = __float2half_rn(v);
+      for (int r = 0; r < 16; ++r) {
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at + r * 128 + lane * 4) : "memory");
+        v += mine[r];
+        if (in && r < rows) {
+          V* o = reinterpret_cast<V*>(places[r + 16]) + col;
+          if constexpr (std::is_same<V, float>::value) *o = v;
+          else if constexpr (std::is_same<V, __half>::value) *o = __float2half_rn(v);
+          else *o = __float2bfloat16_rn(v);
+        }
       }
-    }
+    };
+    if (c.out_dtype == DST_OUT_F32) write(float());
+    else if (c.out_dtype == DST_OUT_BF16) write(__nv_bfloat16());
+    else write(__half());
     __syncwarp();
     if (!SHARED) fetch(step + BS * workers, stage);
     stage = stage + 1 == BS ? 0 : stage + 1;
@@ -1006,12 +1034,12 @@ int launch_cluster(const AdapterCall& c, int64_t max_tiles, cudaStream_t st) {
   return DST_OK;
 }
 
-template <typename T, int RP, int P, bool SHARED_A, bool SHARED_B>
+template <typename T, int RP, int P, bool SHARED>
 int launch_two(AdapterCall c, int64_t max_tiles, cudaStream_t st) {
-  using H = HShape<RP * P, SHARED_A>;
-  using C = CShape<RP, SHARED_B>;
-  auto h_kernel = adapter_h_kernel<T, RP * P, SHARED_A>;
-  auto c_kernel = adapter_columns_kernel<T, RP, P, SHARED_B>;
+  using H = HShape<RP * P, SHARED>;
+  using C = CShape<RP, SHARED>;
+  auto h_kernel = adapter_h_kernel<T, RP * P, SHARED>;
+  auto c_kernel = adapter_columns_kernel<T, RP, P, SHARED>;
   DST_CUDA_TRY(cudaFuncSetAttribute(h_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, H::SMEM));
   DST_CUDA_TRY(cudaFuncSetAttribute(c_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
   const int columns = c.splits;
@@ -1033,10 +1061,9 @@ template <typename T, int RP, int P>
 int launch(const AdapterCall& c, int64_t max_tiles, cudaStream_t st) {
   if (c.ctas) return launch_cluster<T, RP, P>(c, max_tiles, st);
   if constexpr (RP >= 64) {
-    if (c.shared_a) return launch_two<T, RP, P, true, true>(c, max_tiles, st);
-    if (c.shared_b) return launch_two<T, RP, P, false, true>(c, max_tiles, st);
+    if (c.shared) return launch_two<T, RP, P, true>(c, max_tiles, st);
   }
-  return launch_two<T, RP, P, false, false>(c, max_tiles, st);
+  return launch_two<T, RP, P, false>(c, max_tiles, st);
 }
 
 template <typename T>
