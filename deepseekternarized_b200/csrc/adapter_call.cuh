@@ -23,7 +23,7 @@ struct AdapterCall {
   float* h;                   // [splits of K][positions][rows of A]
   int64_t positions;
   int k_splits, share, sub;  // shares of K in the workspace; warps of a row block for h; row blocks of a tile
-  int shared;                 // the row blocks of a tile share A and B
+  int shared_a, shared_b;     // the row blocks of a tile share A, B
   int kind;                   // base and result of the fast forms: 0 float32 / 16 bits, 1 float32 / float32, 2 16 / 16, 3 none / 16; -1: others
   int x_vec;                  // rows of x can be read eight values at a time
 };

@@ -9,11 +9,11 @@ namespace {
 // How a call is cut: CTAs of a cluster (0: two kernels); warps of 16 rows for h inside a CTA and CTAs of them; those for the columns;
 // whether the row blocks of a tile share A and B
 struct Cut {
-  int ctas, share, k_splits, columns, shared;
+  int ctas, share, k_splits, columns, shared_a, shared_b;
 };
 Cut cut_of(int64_t max_tiles, int tile, int64_t K_padded, int64_t N, int rank_padded) {
   const int64_t sms = sm_count(), blocks = max_tiles * (tile / 16);
-  Cut cut{0, 8, 1, 1, 0};
+  Cut cut{0, 8, 1, 1, 0, 0};
   // Up to 48 blocks the cluster's one launch costs the host 5 us less (11 against 16 a call) and the device as much: 1 row of 4096 x
   // 4096 4.2 us against 4.1, 333 rows 8.0 against 8.2, 48 pairs (rank 16 twice) 13.1 against 14.4 with their plan; 64 rows of 37
   // adapters (53 blocks) through 11008 x 4096 14.9 against 11.2. A cluster takes tiles of 16 rows only.
@@ -22,28 +22,30 @@ Cut cut_of(int64_t max_tiles, int tile, int64_t K_padded, int64_t N, int rank_pa
     while (cut.ctas < ADAPTER_MAX_CTAS && max_tiles * cut.ctas * 2 <= 2 * sms) cut.ctas *= 2;
     return cut;
   }
-  // Warps of a block: doubled as long as those of the machine are few, or their steps are many enough to pay for a warp's start. Up
-  // to 8 warps a multiprocessor one step each, up to 16 two, up to 32 five for the columns (32 of them a step); up to 4 one, 12 two,
-  // 22 four for h (64 values of K a step; from rank 64 on a warp counts twice, its sums being long). Best and neighbours by
-  // measurement, us for 1, 2, 4 ... warps (the other product at its best): 64 rows of 37 adapters, 4096 x 11008, rank 32, columns - /
-  // 64.7 / 36.4 / 22.7 / 15.9 / 14.1 / 12.1 (64) / 15.2, h 36.3 / 23.4 / 16.7 / 13.8 / 12.1 / 11.4 (32) / 13.9; 281 rows of 6488 x 1904,
-  // rank 128, columns 67.6 / 44.4 / 32.5 / 26.9 / 23.3 / 21.5 (32) / 24.5, h 74.7 / 46.0 / 32.3 / 24.3 / 21.6 (16) / 24.4; 2000 rows of
-  // 1024 x 1024, rank 16, columns 17.4 / 11.6 / 9.0 / 7.8 / 7.5 (16) / 9.2, h 10.1 / 8.5 / 7.5 / 7.2 (8) / 7.3; 4000 rows of 2048 x
-  // 4096, rank 64, columns 115.7 / 65.7 / 43.5 / 37.5 (8) / 39.6, h 50.6 / 41.1 / 37.4 (4) / 37.8
-  const auto warps = [&](int64_t steps, int weight, int few, int some, int most, int long_run) {
+  // Tiles of 128 rows share B from rank 64 on, and A where there are many: 4000 rows of 2048 x 4096, rank 64, 37.2 us with B shared
+  // against 39.8, rank 128 53 against 60; A shared 37.7 against 37.2, rank 128 57.7 against 54.4, 12 000 rows of 4096 x 4096 98 against
+  // 105 and 190 against 196.
+  cut.shared_b = tile == 128 && rank_padded >= 64, cut.shared_a = cut.shared_b && blocks >= 4 * sms;
+  // Warps of a block: doubled as long as those of the machine are few or their steps many enough to pay for a warp's start. Measured,
+  // us for 1, 2, 4 ... warps with the other product at its best: 64 rows of 37 adapters, 4096 x 11008, rank 32, columns - / 64.7 / 36.4 /
+  // 22.7 / 15.9 / 14.1 / 12.1 (64) / 15.2, h 36.3 / 23.4 / 16.7 / 13.8 / 12.1 / 11.4 (32) / 13.9; 281 rows of 6488 x 1904, rank 128, columns
+  // 67.6 / 44.4 / 32.5 / 26.9 / 23.3 / 21.5 (32) / 24.5, h 74.7 / 46.0 / 32.3 / 24.3 / 21.6 (16) / 24.4; 2000 rows of 1024 x 1024, rank 16,
+  // columns 17.4 / 11.6 / 9.0 / 7.8 / 7.5 (16) / 9.2, h 10.1 / 8.5 / 7.5 / 7.2 (8) / 7.3; 12 000 rows of 4096 x 4096, rank 64, columns
+  // - / 115.6 / 112.2 / 103.2 (8) / 106.6, h 109.1 / 99.4 / 98.0 (4) / 102.6
+  const auto doubled = [](auto more) {
     int n = 1;
-    for (int next = 2; next <= steps; next *= 2) {
-      const int64_t all = blocks * next * weight;
-      const int64_t least = all <= few * sms ? 10 : all <= some * sms ? 18 : 10 * long_run;  // tenths of a step: 60 count as two each for 32
-      if (all > most * sms || steps * 10 < least * next) break;
-      n = next;
-    }
+    while (more((int64_t)n * 2)) n *= 2;
     return n;
   };
-  cut.shared = tile == 128 && rank_padded >= 64;
-  const int h = warps(K_padded / 64, rank_padded >= 64 ? 2 : 1, 4, 12, 22, 4);
-  cut.columns = warps((N + 31) / 32, 1, 8, 16, 32, 5);
-  cut.share = cut.shared ? 1 : std::min(h, 8), cut.k_splits = std::min(cut.shared ? h : std::max(h / 8, 1), 16);
+  const int h = doubled([&](int64_t n) {  // steps of 64 values of K; long sums count twice
+    const int64_t steps = K_padded / 64, all = blocks * n * (rank_padded >= 64 ? 2 : 1);
+    return all <= 22 * sms ? steps >= n * (all <= 4 * sms ? 1 : all <= 12 * sms ? 2 : 4) : n <= 4 && steps >= 16 * n;
+  });
+  cut.columns = doubled([&](int64_t n) {  // steps of 32 columns; the widest shared ones count twice
+    const int64_t steps = (N + 31) / 32, weight = cut.shared_b && rank_padded > 64 ? 2 : 1, all = blocks * n * weight;
+    return all <= 32 * sms ? 10 * steps >= n * (all <= 8 * sms ? 10 : all <= 16 * sms ? 18 : 50) : n <= 8 && steps >= 16 * weight * n;
+  });
+  cut.share = cut.shared_a ? 1 : std::min(h, 8), cut.k_splits = std::min(cut.shared_a ? h : std::max(h / 8, 1), 16);
   return cut;
 }
 
@@ -95,7 +97,7 @@ extern "C" int dst_adapter_apply(const dst_adapters* w, const dst_adapter_rows* 
     else if (out_dtype == own && (!base || base_dtype == own)) c.kind = base ? 2 : 3;
   }
   const Cut cut = cut_of(plan->max_tiles, plan->tile, w->K_padded, w->N, w->rank_padded);
-  c.sub = plan->tile / 16, c.shared = cut.shared, c.ctas = cut.ctas, c.share = cut.share, c.k_splits = cut.k_splits, c.splits = cut.columns;
+  c.sub = plan->tile / 16, c.shared_a = cut.shared_a, c.shared_b = cut.shared_b, c.ctas = cut.ctas, c.share = cut.share, c.k_splits = cut.k_splits, c.splits = cut.columns;
   c.positions = plan->positions, c.h = static_cast<float*>(workspace);
   if (!cut.ctas) {
     if (!workspace || workspace_bytes < dst_adapter_workspace_bytes(w, plan)) return DST_ERR_BAD_ARG;

@@ -1034,12 +1034,12 @@ int launch_cluster(const AdapterCall& c, int64_t max_tiles, cudaStream_t st) {
   return DST_OK;
 }
 
-template <typename T, int RP, int P, bool SHARED>
+template <typename T, int RP, int P, bool SHARED_A, bool SHARED_B>
 int launch_two(AdapterCall c, int64_t max_tiles, cudaStream_t st) {
-  using H = HShape<RP * P, SHARED>;
-  using C = CShape<RP, SHARED>;
-  auto h_kernel = adapter_h_kernel<T, RP * P, SHARED>;
-  auto c_kernel = adapter_columns_kernel<T, RP, P, SHARED>;
+  using H = HShape<RP * P, SHARED_A>;
+  using C = CShape<RP, SHARED_B>;
+  auto h_kernel = adapter_h_kernel<T, RP * P, SHARED_A>;
+  auto c_kernel = adapter_columns_kernel<T, RP, P, SHARED_B>;
   DST_CUDA_TRY(cudaFuncSetAttribute(h_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, H::SMEM));
   DST_CUDA_TRY(cudaFuncSetAttribute(c_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
   const int columns = c.splits;
@@ -1061,9 +1061,10 @@ template <typename T, int RP, int P>
 int launch(const AdapterCall& c, int64_t max_tiles, cudaStream_t st) {
   if (c.ctas) return launch_cluster<T, RP, P>(c, max_tiles, st);
   if constexpr (RP >= 64) {
-    if (c.shared) return launch_two<T, RP, P, true>(c, max_tiles, st);
+    if (c.shared_a && c.shared_b) return launch_two<T, RP, P, true, true>(c, max_tiles, st);
+    if (c.shared_b) return launch_two<T, RP, P, false, true>(c, max_tiles, st);
   }
-  return launch_two<T, RP, P, false>(c, max_tiles, st);
+  return launch_two<T, RP, P, false, false>(c, max_tiles, st);
 }
 
 template <typename T>

@@ -476,9 +476,9 @@ def some_slots(rows, n, g):
 @gpu
 @pytest.mark.parametrize("dtype,base,out", [(BF16, F32, BF16), (BF16, F32, F32), (BF16, BF16, BF16), (F16, F32, F16), (F16, F16, F16), (F16, F32, F32),
                                             (BF16, None, None), (F16, None, None), (BF16, F16, F32)])
-@pytest.mark.parametrize("rows,r", [(900, 8), (900, 20), (900, 64), (900, 100), (3100, 16), (3100, 64), (3100, 128)])
+@pytest.mark.parametrize("rows,r", [(900, 8), (900, 20), (900, 64), (900, 100), (3100, 16), (3100, 64), (3100, 128), (9700, 64), (9700, 100)])
 def test_adapters_of_many_rows(rows, r, dtype, base, out):
-    """More blocks of rows than a cluster takes; from 2960 rows on in tiles of 128, which share A and B at the higher ranks."""
+    """More blocks of rows than a cluster takes; from 2960 rows on in tiles of 128, which share B at the higher ranks, many A too."""
     K, N = 320, 264
     A, B, scale, ad = make(2, K, N, r, dtype, rows)
     g = gen(rows + r)
@@ -494,7 +494,7 @@ def test_adapters_of_many_rows(rows, r, dtype, base, out):
 
 @gpu
 @pytest.mark.parametrize("K,N", [(1, 1), (7, 3), (33, 31), (64, 33), (129, 200), (1000, 70), (2049, 513)])
-@pytest.mark.parametrize("rows", [850, 2970])
+@pytest.mark.parametrize("rows", [850, 2970, 9601])
 def test_adapters_of_many_rows_and_odd_sizes(rows, K, N):
     for dtype, out, r in ((BF16, BF16, 5), (F16, F32, 20), (BF16, F32, 64), (F16, F16, 128)):
         A, B, scale, ad = make(2, K, N, r, dtype, K + N)
@@ -505,7 +505,7 @@ def test_adapters_of_many_rows_and_odd_sizes(rows, K, N):
 
 @gpu
 @pytest.mark.parametrize("N,r", [(128, 8), (66, 16), (6, 3), (640, 64), (200, 32), (400, 50)])
-@pytest.mark.parametrize("rows", [900, 3000])
+@pytest.mark.parametrize("rows", [900, 3000, 9500])
 def test_adapters_of_many_rows_in_two_parts(rows, N, r):
     A, B, scale, ad = make(2, 160, N, r, BF16, N, parts=2)
     g = gen(N)
@@ -515,7 +515,7 @@ def test_adapters_of_many_rows_in_two_parts(rows, N, r):
 
 
 @gpu
-@pytest.mark.parametrize("rows,r", [(900, 8), (900, 64), (3000, 8), (3000, 64), (3000, 128)])
+@pytest.mark.parametrize("rows,r", [(900, 8), (900, 64), (3000, 8), (3000, 64), (3000, 128), (9500, 64), (9500, 128)])
 def test_adapters_of_many_rows_at_any_stride(rows, r):
     K, N = 200, 168
     A, B, scale, ad = make(2, K, N, r, BF16, 1)
@@ -534,7 +534,7 @@ def test_adapters_of_many_rows_at_any_stride(rows, r):
 
 @gpu
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("rows,r", [(900, 16), (3000, 64)])
+@pytest.mark.parametrize("rows,r", [(900, 16), (3000, 64), (9500, 64)])
 def test_many_rows_keep_to_themselves(rows, r, dtype):
     """NaNs and infinities in some rows leave the others as they were; a second call gives the same."""
     A, B, scale, ad = make(2, 256, 128, r, dtype, 3)
@@ -857,7 +857,7 @@ def test_adapted_standard_layer_and_dropped_ids():
 
 
 @gpu
-@pytest.mark.parametrize("T,r", [(48, 16), (1000, 16), (3000, 64)])
+@pytest.mark.parametrize("T,r", [(48, 16), (1000, 16), (3000, 64), (9500, 64)])
 def test_captured_steps_follow_their_inputs(T, r):
     """Router, plan and adapters in one captured graph: replayed on other logits, rows and requests, another adapter loaded."""
     E, n, K, N = 64, 4, 256, 128
