@@ -148,8 +148,8 @@ class B200Ops:
             if bias.numel() != E:
                 raise ValueError("the gate bias holds one value per expert")
             p_bias = bias.data_ptr()
-        w = torch.empty((T, top_k), dtype=torch.float32, device=dev)
-        ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+        w = torch.empty(T, top_k, dtype=torch.float32, device=dev)
+        ids = torch.empty(T, top_k, dtype=torch.int32, device=dev)
         with kb._guard(dev):
             rc = lib.dst_route_group_topk(logits.data_ptr(), code, stride, p_bias, T, E, n_groups, n_groups if topk_groups is None else topk_groups,
                                           _lib.GROUP_SCORES[group_score], top_k, _lib.SCORE_FUNCS[score_func], gate_temp, 1 if renorm else 0,

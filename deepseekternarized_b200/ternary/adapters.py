@@ -263,7 +263,7 @@ class LowRankAdapters:
             p_base = base.data_ptr()
         out_stride = N
         if out is None:
-            out = torch.empty((P, N), dtype=out_dtype or (base.dtype if base is not None else x.dtype), device=dev)
+            out = torch.empty(P, N, dtype=out_dtype or (base.dtype if base is not None else x.dtype), device=dev)
         elif out.shape != (P, N) or (out_dtype is not None and out.dtype != out_dtype) or out.device != dev \
                 or (P > 0 and out.stride(1) != 1 and N > 1) or (P > 1 and out.stride(0) < N):
             raise RuntimeError("the result is float32, bf16 or fp16 [rows, N]")
