@@ -64,6 +64,11 @@ __device__ __forceinline__ double score64(double z, double mx, double sum) {
   return sqrt(fmax(z, 0.0) + log1p(exp(-fabs(z))));  // a NaN comes through log1p
 }
 
+template <int SCORE>
+__device__ __noinline__ double score64_of_lane(double z, double mx) {
+  return score64<SCORE>(z, mx, 1.0);
+}
+
 // A token in 64 bits by the whole block, its keys in shared memory (`keys` [E]). Few tokens come here, but the kernel ends with the
 // last of them: the evaluations of a thread overlap, and a lane looks at its run of keys eight at a time.
 template <int SCORE>
@@ -164,14 +169,25 @@ __device__ __noinline__ void route_exact(const GroupRoute& a, int64_t t, uint64_
 
 // float32 scores: near ones for the selection, which allows for their errors (units of 2^-24 of the score: the hardware's
 // exponential 4 and 2 |z| for its argument, reciprocal and square root 2 each), and those of the picks, for the weights.
-// log(1 + e) = 2 artanh(e / (2 + e)) = 2 (t + t^3 / 3 + t^5 / 5 + ...), t <= 1 / 3: seven terms leave 2e-8 of it.
+// log(1 + e) = 2 artanh(e / (2 + e)) = 2 (t + t^3 / 3 + t^5 / 5 + ...), t <= 1 / 3: seven terms leave 2e-8 of it. The instructions'
+// forms that take subnormal numbers for zeros: 1e-19 of a score at most, and a third of the instructions fewer.
+__device__ __forceinline__ float exp_near(float z) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(z * 1.44269504f));
+  return r;
+}
+__device__ __forceinline__ float inverse_near(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 template <int SCORE>
 __device__ __forceinline__ float score_near(float z) {
-  if (SCORE == DST_SCORE_SIGMOID) return __fdividef(1.f, 1.f + __expf(-z));
-  const float e = __expf(-fabsf(z)), t = __fdividef(e, 2.f + e), u = t * t;
+  if (SCORE == DST_SCORE_SIGMOID) return inverse_near(1.f + exp_near(-z));
+  const float e = exp_near(-fabsf(z)), t = e * inverse_near(2.f + e), u = t * t;
   const float p = fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, 2.f / 13.f, 2.f / 11.f), 2.f / 9.f), 2.f / 7.f), 2.f / 5.f), 2.f / 3.f), 2.f);
   float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(fmaf(t, p, fmaxf(z, 0.f))));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(t, p, fmaxf(z, 0.f))));
   return r;
 }
 template <int SCORE>
@@ -284,13 +300,13 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
       float z[8];
       eight(j0, z);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += j0 + i < n ? __expf(z[i] * inv_temp - mx) : 0.f;
+      for (int i = 0; i < 8; ++i) sum += j0 + i < n ? exp_near(z[i] * inv_temp - mx) : 0.f;
     }
 #pragma unroll
     for (int off = LPT / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(FULL, sum, off);
     inv_sum = 1.f / sum;
   }
-  const auto near = [&](float v) { return SCORE == DST_SCORE_SOFTMAX ? __expf(v * inv_temp - mx) * inv_sum : score_near<SCORE>(v * inv_temp); };
+  const auto near = [&](float v) { return SCORE == DST_SCORE_SOFTMAX ? exp_near(v * inv_temp - mx) * inv_sum : score_near<SCORE>(v * inv_temp); };
 
   uint32_t top[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   float special_key = 0.f;
@@ -358,7 +374,7 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
 
   const auto key64 = [&](float z, float b) {  // softmax: without the division by the sum of all, for comparisons without a bias
     const double v = a.temp == 1.f ? (double)z : (double)z / (double)a.temp;
-    return score64<SCORE>(v, SCORE == DST_SCORE_SOFTMAX ? (double)zmax / fabs((double)a.temp) : 0.0, 1.0) + (double)b;
+    return score64_of_lane<SCORE>(v, SCORE == DST_SCORE_SOFTMAX ? (double)zmax / fabs((double)a.temp) : 0.0) + (double)b;
   };
 
   // groups
@@ -393,26 +409,29 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
         if (__any_sync(FULL, look)) {
           // The close groups in 64 bits; they share the places that those among them had. A lane looks at its two largest keys; a
           // third that may be among its group's largest: the other form.
-          double v1 = -INFINITY, v2 = -INFINITY;
-          bool lost = false;
-          if (look && close) {
-            if (!a.bias) {  // by the logits, which are exact
-              const float z1 = value_of(m1), z2 = value_of(m2);
-              v1 = key64(flip ? -z1 : z1, 0.f), v2 = key64(flip ? -z2 : z2, 0.f);
-            } else {
-              const float least = value_of(sums ? m2 : m1), reach = 2.f * delta + 0x1p-22f * fabsf(least);
-              const auto may = [&](uint32_t k) { return k && !(least - value_of(k) > reach); };
-              lost = may(top[2]);
-              bool first = may(top[0]), second = may(top[1]);
-              for (int j = 0; j < n && (first || second); ++j) {
-                const bool is_first = first && own[j] == top[0];
-                if (is_first || (second && own[j] == top[1])) {
-                  const double k = key64(load_logit(a, row + id0 + j), a.bias[id0 + j]);
-                  v2 = fmax(v2, fmin(v1, k)), v1 = fmax(v1, k);
-                  (is_first ? first : second) = false;
-                }
-              }
+          bool has1 = look && close, has2 = has1, lost = false;
+          float z1 = value_of(m1), z2 = value_of(m2), b1 = 0.f, b2 = 0.f;  // without a bias: the group's two logits, which are exact
+          if (flip) z1 = -z1, z2 = -z2;
+          if (a.bias && has1) {
+            const float least = value_of(sums ? m2 : m1), reach = 2.f * delta + 0x1p-22f * fabsf(least);
+            const auto may = [&](uint32_t k) { return k && !(least - value_of(k) > reach); };
+            lost = may(top[2]), has1 = may(top[0]), has2 = may(top[1]);
+            int at1 = -1, at2 = -1;
+            for (int j = n - 1; j >= 0; --j) {
+              const uint32_t k = own[j];
+              if (k == top[1]) at2 = j;
+              if (k == top[0]) at1 = j;
             }
+            if (top[0] == top[1])  // the second one of that number
+              for (at2 = at1 + 1; at2 < n - 1 && own[at2] != top[1];) ++at2;
+            if (has1) z1 = load_logit(a, row + id0 + at1), b1 = a.bias[id0 + at1];
+            if (has2) z2 = load_logit(a, row + id0 + at2), b2 = a.bias[id0 + at2];
+          }
+          double v1 = -INFINITY, v2 = -INFINITY;
+          if (has1) v1 = key64(z1, b1);
+          if (has2) {
+            const double k = key64(z2, b2);
+            v2 = fmin(v1, k), v1 = fmax(v1, k);
           }
           if (a.bias) {
             for (int off = 1; off < (1 << a.shift); off <<= 1) {
@@ -524,8 +543,11 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
           if (own[j] == top[0] && skip-- == 0) next = j;
       const int extra_id = id0 + next;
       const float extra_z = extra ? load_logit(a, row + extra_id) : 0.f;
-      const uint64_t own_key = pick ? order_of(key64(flip ? -zi : zi, b)) : 0;
-      const uint64_t extra_key = extra ? order_of(key64(extra_z, a.bias[extra_id])) : 0;
+      // one evaluation for both where no lane has a pick and an extra one
+      uint64_t own_key = 0, extra_key = 0;
+      if (near_picks && (pick || extra)) own_key = order_of(key64(pick ? (flip ? -zi : zi) : extra_z, pick ? b : a.bias[extra_id]));
+      if (extra && pick) extra_key = order_of(key64(extra_z, a.bias[extra_id]));
+      if (extra && !pick) extra_key = own_key, own_key = 0;
       int own_rank = 0, extra_rank = 0;
       const auto against = [&](uint64_t key, int e) {
         own_rank += key > own_key || (key == own_key && e < id);
