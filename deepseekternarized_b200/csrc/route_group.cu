@@ -461,6 +461,8 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
 
   uint32_t number = 0, before = 0;  // of pick `tl`; of the round before
   int from = 0, win_before = -1, run = 0, nth = 0;  // the lane that had it, as its run-th of that number
+  uint32_t popped = 0;                              // the lane's own last pick, as its same-th of that number
+  int same = 0;
   for (int r = 0; r < a.top_k; ++r) {
     const uint32_t best = seg_max(top[0]);
     const int win = __ffs(__ballot_sync(FULL, top[0] == best) & segment) - 1;
@@ -468,6 +470,7 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
     before = best, win_before = win;
     if (tl == r) number = best, from = win, nth = run;
     if (lane == win) {
+      same = top[0] == popped ? same + 1 : 1, popped = top[0];
 #pragma unroll
       for (int i = 0; i < 7; ++i) top[i] = top[i + 1];
       top[7] = 0;
@@ -475,20 +478,23 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
   }
   const bool pick = tl < a.top_k;
   from &= LPT - 1;
-  int at = 0;
   __syncwarp();
-  const uint32_t* theirs = mine + from * a.stride_s;
-  for (int j0 = ((a.chunk - 1) & ~3); j0 >= 0; j0 -= 4) {  // from behind: the match that is left at the end is the first
-    const uint4 v = *reinterpret_cast<const uint4*>(theirs + j0);
-    at = v.w == number ? j0 + 3 : at;
-    at = v.z == number ? j0 + 2 : at;
-    at = v.y == number ? j0 + 1 : at;
-    at = v.x == number ? j0 : at;
-  }
-  for (; nth > 0; --nth) {
-    ++at;
-    while (at < a.chunk - 1 && theirs[at] != number) ++at;
-  }
+  const auto place_of = [&](const uint32_t* of, uint32_t value, int nth) {  // of the nth one of that number (0: the first)
+    int at = 0;
+    for (int j0 = ((a.chunk - 1) & ~3); j0 >= 0; j0 -= 4) {  // from behind: the match that is left at the end is the first
+      const uint4 v = *reinterpret_cast<const uint4*>(of + j0);
+      at = v.w == value ? j0 + 3 : at;
+      at = v.z == value ? j0 + 2 : at;
+      at = v.y == value ? j0 + 1 : at;
+      at = v.x == value ? j0 : at;
+    }
+    for (; nth > 0; --nth) {
+      ++at;
+      while (at < a.chunk - 1 && of[at] != value) ++at;
+    }
+    return at;
+  };
+  const int at = place_of(mine + from * a.stride_s, number, nth);
   const int id = min((from >> a.shift) * a.size + (from & ((1 << a.shift) - 1)) * a.chunk + at, a.E - 1);
   float zi = pick ? load_logit(a, row + id) : 0.f;
   if (flip) zi = -zi;
@@ -499,20 +505,29 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
     const float key = value_of(number), b = pick ? a.bias[id] : 0.f;
     const float tol = 2.f * delta + 0x1p-22f * fabsf(key);
     const float next_key = __shfl_down_sync(FULL, key, 1, LPT), next_z = __shfl_down_sync(FULL, zi, 1, LPT), next_b = __shfl_down_sync(FULL, b, 1, LPT);
-    const bool unsure = tl + 1 < a.top_k && !(key - next_key > tol) && !(zi == next_z && b == next_b);
+    const bool near_next = tl + 1 < a.top_k && !(key - next_key > tol);
+    bool near_picks = seg_any(near_next && !(zi == next_z && b == next_b));
     // and the last one above what is left; a lane whose list ran out may have had more
     const float last = __shfl_sync(FULL, key, a.top_k - 1, LPT), last_tol = __shfl_sync(FULL, tol, a.top_k - 1, LPT);
     const uint32_t left = seg_max(top[0]);
     const int first_from = __shfl_sync(FULL, from, 0, LPT);
     const bool one_lane = !seg_any(pick && from != first_from);
-    const bool any_unsure = seg_any(unsure);
     again = again || (a.top_k == 8 && a.chunk > 8 && one_lane);
-    bool near_picks = any_unsure;
     const bool border = left && !(last - value_of(left) > last_tol);
-    if (__any_sync(FULL, border && !again)) {  // equal logits and biases at the border are no matter
+    bool extra = false, several = false;  // the lane's next one is as near as the last pick; and another of its own
+    int extra_id = 0;
+    float extra_z = 0.f, extra_b = 0.f;
+    if (__any_sync(FULL, border && !again)) {
+      extra = border && !again && top[0] && !(last - value_of(top[0]) > last_tol);
+      several = extra && (top[1] ? !(last - value_of(top[1]) > last_tol) : n > 8);
+      if (extra) {
+        extra_id = min(id0 + place_of(own, top[0], popped == top[0] ? same : 0), a.E - 1);
+        extra_z = load_logit(a, row + extra_id), extra_b = a.bias[extra_id];
+      }
+      // equal logits and biases at the border are no matter
       const float last_z = __shfl_sync(FULL, zi, a.top_k - 1, LPT), last_b = __shfl_sync(FULL, b, a.top_k - 1, LPT);
-      bool other = false;
-      if (border && top[0])
+      bool other = extra && ((flip ? -extra_z : extra_z) != last_z || extra_b != last_b);
+      if (several)
         for (int j = 0; j < n; ++j) {
           const float k = value_of(own[j]);
           if (!(last - k > last_tol) && !(k - last > last_tol)) {
@@ -527,27 +542,19 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
     if (SCORE == DST_SCORE_SOFTMAX) {
       again = again || near_picks;  // the sum of all scores would be needed in 64 bits
     } else if (__any_sync(FULL, near_picks)) {
-      // The picks and, of each lane, the next one where it is as near as the last pick, in 64 bits: each takes the place of its rank
-      // among them. Two such in a lane, or a list that has run out behind the first: the other form.
-      const bool extra = near_picks && top[0] && !(last - value_of(top[0]) > last_tol);
-      const bool any_more = seg_any(extra && (top[1] ? !(last - value_of(top[1]) > last_tol) : n > 8));
+      // The picks that are near another or the border and the extra ones in 64 bits, the others as they are: each takes the place of its
+      // rank among them. Several extra ones in a lane: the other form.
+      const bool any_more = seg_any(near_picks && several);
       again = again || any_more;
-      int skip = 0, next = 0;  // the extra one is the lane's first of its number behind the lane's picks of that number
-      for (int r = 0; r < a.top_k; ++r) {
-        const uint32_t o = __shfl_sync(FULL, number, r, LPT);
-        const int f = __shfl_sync(FULL, from, r, LPT);
-        skip += o == top[0] && f == tl;
+      const bool near_last = __shfl_up_sync(FULL, near_next, 1, LPT) && tl > 0;
+      const bool look = near_picks && pick && (near_next || near_last || (border && !(key - value_of(left) > tol)));
+      extra = extra && near_picks;
+      uint64_t own_key = pick ? order_of((double)key) : 0, extra_key = 0;
+      if (look || extra) {  // one evaluation for both where no lane has both
+        const uint64_t k = order_of(key64(look ? (flip ? -zi : zi) : extra_z, look ? b : extra_b));
+        (look ? own_key : extra_key) = k;
       }
-      if (extra)
-        for (int j = 0; j < n; ++j)
-          if (own[j] == top[0] && skip-- == 0) next = j;
-      const int extra_id = id0 + next;
-      const float extra_z = extra ? load_logit(a, row + extra_id) : 0.f;
-      // one evaluation for both where no lane has a pick and an extra one
-      uint64_t own_key = 0, extra_key = 0;
-      if (near_picks && (pick || extra)) own_key = order_of(key64(pick ? (flip ? -zi : zi) : extra_z, pick ? b : a.bias[extra_id]));
-      if (extra && pick) extra_key = order_of(key64(extra_z, a.bias[extra_id]));
-      if (extra && !pick) extra_key = own_key, own_key = 0;
+      if (look && extra) extra_key = order_of(key64(extra_z, extra_b));
       int own_rank = 0, extra_rank = 0;
       const auto against = [&](uint64_t key, int e) {
         own_rank += key > own_key || (key == own_key && e < id);
@@ -558,10 +565,11 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
         const int e = __shfl_sync(FULL, id, r, LPT);
         against(k, e);
       }
-      for (int r = 0; r < LPT; ++r) {
-        const uint64_t k = __shfl_sync(FULL, extra_key, r, LPT);
-        const int e = __shfl_sync(FULL, extra_id, r, LPT);
-        if (k) against(k, e);
+      for (unsigned rest = __ballot_sync(FULL, extra) & segment; __any_sync(FULL, rest != 0); rest &= rest - 1) {
+        const int who = rest ? __ffs(rest) - 1 : lane;
+        const uint64_t k = __shfl_sync(FULL, extra_key, who);
+        const int e = __shfl_sync(FULL, extra_id, who);
+        if (rest) against(k, e);
       }
       settled = near_picks && !again;
       const bool own_in = pick && own_rank < a.top_k, extra_in = extra && extra_rank < a.top_k;
