@@ -7,11 +7,16 @@
 //   picks                        the top_k largest keys among the kept groups' experts (equal keys: the lower id), in that order
 //   weight_i = s of pick i, divided by the picks' sum + 1e-20 when renormalised (top_k > 1), times route_scale
 //
-// The picks are those of exact arithmetic. Without a bias f keeps the order of the logits, which decide by themselves; sums of two
-// scores and keys with a bias are compared in float32 where they are further apart than their rounding errors can reach. Groups and
-// picks that are closer are told apart in 64 bits by themselves; where that takes a sum over all experts (softmax with a bias) or
-// there are many of them, the token is done again in 64 bits by its block, which costs that 4 to 7 us (256 experts). A NaN ranks
-// above every number (such a token goes that way too), so a token's ids are distinct and inside [0, E) whatever the logits hold.
+// The picks are those of exact arithmetic, as far as 64 bits tell. Without a bias f keeps the order of the logits, which decide by
+// themselves; sums of two scores and keys with a bias are compared in float32 where they are further apart than their rounding errors
+// can reach. Groups and picks that are closer are told apart in 64 bits by themselves (one in some hundred tokens; 1 to 2 us at the end
+// of a call); where that takes a sum over all experts (softmax with a bias) or there are many of them, the token is done again in 64
+// bits by its block, which costs that 4 to 7 us (256 experts). A NaN ranks above every number (such a token goes that way too), so a
+// token's ids are distinct and inside [0, E) whatever the logits hold.
+//
+// What bounds it: latency for few tokens (launch, load, a sort and eight rounds in a row), instructions for many: 60 an expert and warp,
+// a third of them its score, a seventh the sorting; 16 384 tokens of 384 experts run as one wave of warps in 21 us, their traffic would
+// take 4.
 #include "dst_common.cuh"
 
 namespace dst {
@@ -645,9 +650,9 @@ template <int SCORE>
 int launch_for(const GroupRoute& a, cudaStream_t st) {
   // A warp for each token where that is a dozen of them a multiprocessor; then several tokens a warp, which share the steps across
   // lanes. Eight groups, us for 777 / 2000 / 4736 / 16 384 tokens: 384 experts, top-6, square roots of softplus, sums and a bias: a
-  // warp each 8.5 / 10.8 / 17.2 / 38.2, two a warp 9.2 / 10.4 / 15.5 / 28.4, four 11.9 / 12.9 / 18.6 / 27.3; 256 experts, top-8,
-  // sigmoid, sums and a bias: 6.5 / 8.8 / 13.6 / 26.6, 7.2 / 9.0 / 12.0 / 21.5, 7.3 / 8.9 / 11.8 / 19.4; by the largest, without a
-  // bias: 4.4 / 5.6 / 8.5 / 19.5, 4.6 / 5.3 / 6.9 / 15.0, 4.6 / 4.8 / 5.7 / 11.3
+  // warp each 7.2 / 9.1 / 14.5 / 33.8, two a warp 7.7 / 8.9 / 11.5 / 23.9, four 10.6 / 11.4 / 13.1 / 21.3; 256 experts, top-8,
+  // sigmoid, sums and a bias: 5.6 / 7.5 / 11.0 / 24.2, 6.5 / 7.9 / 9.3 / 19.1, 7.3 / 8.2 / 9.2 / 16.3; by the largest, without a
+  // bias: 4.3 / 5.6 / 8.7 / 20.5, 4.5 / 5.1 / 6.8 / 15.1, 4.6 / 4.7 / 6.1 / 11.7
   const int64_t sms = sm_count();
   if (a.groups > 16 || a.T <= 12 * sms) return launch<SCORE, 32>(a, st);
   if (a.groups > 8 || a.E > 512 || a.T <= 32 * sms) return launch<SCORE, 16>(a, st);

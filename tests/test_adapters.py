@@ -33,12 +33,13 @@ def gen(seed):
 
 # ------------------------------------------------------------------------------------------------- routing in groups
 def route64(logits, k, scale, renorm, score, bias, temp, groups, kept, group_score):
-    """The definition on the CPU in 64 bits; NaN first, equal keys by the lower index."""
-    v = logits.double().cpu() / float(np.float32(temp))
+    """The definition in 64 bits; NaN first, equal keys by the lower index. (On the GPU: the CPU's vectorised functions round equal
+    numbers differently at the end of a run.)"""
+    v = logits.double() / float(np.float32(temp))
     T, E = v.shape
     s = {"softmax": lambda: torch.softmax(v, -1), "sigmoid": lambda: torch.sigmoid(v),
          "sqrtsoftplus": lambda: torch.logaddexp(v, torch.zeros_like(v)).sqrt()}[score]()
-    key = s if bias is None else s + bias.double().cpu()
+    key = s if bias is None else s + bias.double()
     size = E // groups
 
     def first(values):  # positions in descending order
@@ -46,12 +47,12 @@ def route64(logits, k, scale, renorm, score, bias, temp, groups, kept, group_sco
 
     best = key.view(T, groups, size).sort(dim=-1, descending=True).values[..., :2 if group_score == "top2" else 1].sum(-1)
     allowed = first(best)[:, :kept].sort(dim=-1).values
-    cand = (allowed[..., None] * size + torch.arange(size)).flatten(1)
+    cand = (allowed[..., None] * size + torch.arange(size, device=DEV)).flatten(1)
     ids = cand.gather(1, first(key.gather(1, cand))[:, :k])
     w = s.gather(1, ids)
     if renorm and k > 1:
         w = w / (w.sum(-1, keepdim=True) + 1e-20)
-    return (w * scale).numpy(), ids.numpy()
+    return (w * scale).cpu().numpy(), ids.cpu().numpy()
 
 
 def check_route(logits, k, scale=1.0, renorm=True, score="sigmoid", bias=None, temp=1.0, groups=8, kept=4, group_score="top2"):
