@@ -71,10 +71,9 @@ __device__ __forceinline__ uint16_t piece(float& v, __half) {
   return h;
 }
 
-__device__ __forceinline__ float element(const void* p, int64_t i, int dtype) {
-  if (dtype == DST_OUT_F32) return static_cast<const float*>(p)[i];
-  if (dtype == DST_OUT_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  return __half2float(static_cast<const __half*>(p)[i]);
+// A value of base as it lies there: reading several before the first is used keeps them all on their way.
+__device__ __forceinline__ float of_raw(uint32_t v, int dtype) {
+  return dtype == DST_OUT_F32 ? __uint_as_float(v) : dtype == DST_OUT_BF16 ? __uint_as_float(v << 16) : __half2float(__ushort_as_half((uint16_t)v));
 }
 
 // Four values of a row and their sum with what `base` holds of it
@@ -94,16 +93,15 @@ __device__ __forceinline__ uint2 pack4(const float* v) {
   return make_uint2(w[0], w[1]);
 }
 
-// base + v for up to four neighbouring columns, of any types and alignment
-__device__ __forceinline__ void finish_single(const AdapterCall& c, int64_t row, int64_t col, int n, const float* v) {
+// v for up to four neighbouring columns, of any type and alignment
+__device__ __forceinline__ void store_single(const AdapterCall& c, int64_t row, int64_t col, int n, const float* v) {
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     if (j < n) {
-      const int64_t bi = row * c.base_stride + col + j, oi = row * c.out_stride + col + j;
-      const float r = c.base ? v[j] + element(c.base, bi, c.base_dtype) : v[j];
-      if (c.out_dtype == DST_OUT_F32) static_cast<float*>(c.out)[oi] = r;
-      else if (c.out_dtype == DST_OUT_BF16) static_cast<__nv_bfloat16*>(c.out)[oi] = __float2bfloat16_rn(r);
-      else static_cast<__half*>(c.out)[oi] = __float2half_rn(r);
+      const int64_t o = row * c.out_stride + col + j;
+      if (c.out_dtype == DST_OUT_F32) static_cast<float*>(c.out)[o] = v[j];
+      else if (c.out_dtype == DST_OUT_BF16) static_cast<__nv_bfloat16*>(c.out)[o] = __float2bfloat16_rn(v[j]);
+      else static_cast<__half*>(c.out)[o] = __float2half_rn(v[j]);
     }
 }
 
@@ -427,16 +425,32 @@ __global__ void __launch_bounds__(WARPS * 32, RP* P <= 64 ? 2 : 1) adapter_kerne
     for (int step = worker; step < steps; step += workers) {
       uint4 bn[KB][4];
       load_b(step + workers, bn);
+      const int col = column(step), left = behind(step, col) - 4 * q;
+      uint32_t raw[2][2][4] = {};
+      const auto read = [&](auto type) {  // behind the last column: that one again
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              raw[half][i][j] = static_cast<const decltype(type)*>(c.base)[(half ? ob : oa) * c.base_stride + col + 4 * q + min(16 * i + j, left - 1)];
+      };
+      if (c.base && es == 4) read(uint32_t());
+      else if (c.base) read(uint16_t());
       float d[4][4];
       product(Int<BF ? 3 : 2>(), P == 2 && step >= per_part, d);
-      const int col = column(step), left = behind(step, col) - 4 * q;
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           if ((half ? vb : va) && left > 16 * i) {
-            const float v[4] = {d[2 * i][2 * half], d[2 * i][2 * half + 1], d[2 * i + 1][2 * half], d[2 * i + 1][2 * half + 1]};
-            finish_single(c, half ? ob : oa, col + 4 * q + 16 * i, min(4, left - 16 * i), v);
+            float v[4] = {d[2 * i][2 * half], d[2 * i][2 * half + 1], d[2 * i + 1][2 * half], d[2 * i + 1][2 * half + 1]};
+            if (c.base) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) v[j] += of_raw(raw[half][i][j], c.base_dtype);
+            }
+            store_single(c, half ? ob : oa, col + 4 * q + 16 * i, min(4, left - 16 * i), v);
           }
       next_b(bn);
     }
@@ -937,26 +951,17 @@ __global__ void __launch_bounds__(256, RP <= 64 ? 2 : 1) adapter_columns_kernel(
     places[lane + 16] = static_cast<char*>(c.out) + row_at(lane) * c.out_stride * (c.out_dtype == DST_OUT_F32 ? 4 : 2);
   }
   __syncwarp();
-  float next[16];
-  const auto base_of = [&](int step) {
-    const int64_t col = column(step) + lane;
-    const bool in = c.base && step < steps && col < (P == 2 && step < per_part ? Np : N);
+  uint32_t next[16] = {};
+  const auto base_of = [&](int step) {  // behind the last step and column: the last ones again
+    if (!c.base) return;
+    const int at = min(step, steps - 1);
+    const int64_t col = min(column(at) + lane, (P == 2 && at < per_part ? Np : N) - 1);
     const auto read = [&](auto type) {
-      using V = decltype(type);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        next[r] = 0.f;
-        if (in && r < rows) {
-          const V v = reinterpret_cast<const V*>(places[r])[col];
-          if constexpr (std::is_same<V, float>::value) next[r] = v;
-          else if constexpr (std::is_same<V, __half>::value) next[r] = __half2float(v);
-          else next[r] = __bfloat162float(v);
-        }
-      }
+      for (int r = 0; r < 16; ++r) next[r] = reinterpret_cast<const decltype(type)*>(places[r])[col];
     };
-    if (c.base_dtype == DST_OUT_F32) read(float());
-    else if (c.base_dtype == DST_OUT_BF16) read(__nv_bfloat16());
-    else read(__half());
+    if (c.base_dtype == DST_OUT_F32) read(uint32_t());
+    else read(uint16_t());
   };
   const auto fetch = [&](int step, int stage) {
     if (step < steps) fetch_b(b + (int64_t)column(step) * RP, stage);
@@ -979,7 +984,7 @@ __global__ void __launch_bounds__(256, RP <= 64 ? 2 : 1) adapter_columns_kernel(
     zero(d);
     product(NP(), stage, d);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) mine[r] = next[r];
+    for (int r = 0; r < 16; ++r) mine[r] = c.base ? of_raw(next[r], c.base_dtype) : 0.f;
     base_of(step + workers);
     const uint32_t at = part0 + stage * S::BST;
 #pragma unroll
