@@ -16,7 +16,7 @@ Cut cut_of(int64_t max_tiles, int tile, int64_t K_padded, int64_t N, int rank_pa
   Cut cut{0, 8, 1, 1, 0, 0};
   // Up to 48 blocks the cluster's one launch costs the host 5 us less (11 against 16 a call) and the device as much: 1 row of 4096 x
   // 4096 4.2 us against 4.1, 333 rows 8.0 against 8.2, 48 pairs (rank 16 twice) 13.1 against 14.4 with their plan; 64 rows of 37
-  // adapters (53 blocks) through 11008 x 4096 14.9 against 11.2. A cluster takes tiles of 16 rows only.
+  // adapters (53 blocks) through 4096 x 11008 14.9 against 10.8. A cluster takes tiles of 16 rows only.
   if (tile == 16 && blocks <= 48) {
     cut.ctas = 1;
     while (cut.ctas < ADAPTER_MAX_CTAS && max_tiles * cut.ctas * 2 <= 2 * sms) cut.ctas *= 2;
