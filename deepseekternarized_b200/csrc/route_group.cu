@@ -268,7 +268,7 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
     }
   }
   // The lane's numbers in blocks of eight. A logit is negated under a negative temperature: experts rank by it as they do by their
-  // scores. On the way: the largest magnitude, softmax's largest, and `special`, a NaN from anything that is not finite.
+  // scores. On the way: the largest, softmax's largest magnitude, and `special`, a NaN from anything that is not finite.
   const bool flip = a.temp < 0.f;
   const float inv_temp = 1.f / fabsf(a.temp);
   float zmax = -INFINITY, zabs = 0.f, special = 0.f, inv_sum = 1.f, mx = 0.f;
@@ -288,8 +288,8 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
   const auto range = [&](const float (&z)[8], bool numbers) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (SCORE == DST_SCORE_SOFTMAX) zmax = fmaxf(zmax, z[i]);
-      zabs = fmaxf(zabs, fabsf(z[i]));
+      if (SCORE != DST_SCORE_SIGMOID) zmax = fmaxf(zmax, z[i]);
+      if (SCORE == DST_SCORE_SOFTMAX) zabs = fmaxf(zabs, fabsf(z[i]));
       if (numbers) special = fmaf(z[i], 0.f, special);
     }
   };
@@ -319,7 +319,7 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
     float z[8];
     eight(j0, z);
     if (SCORE != DST_SCORE_SOFTMAX) range(z, !a.bias);
-    if (a.bias) {  // a NaN shows in the key, an infinity in zabs
+    if (a.bias) {  // a NaN shows in the key, as does an infinite score
       float b[8];
       if (a.vec_bias) {
         const float4 u = __ldg(reinterpret_cast<const float4*>(a.bias + id0 + j0)), v = __ldg(reinterpret_cast<const float4*>(a.bias + id0 + j0 + 4));
@@ -353,28 +353,29 @@ __device__ __forceinline__ bool route_tokens(const GroupRoute& a, int64_t t, boo
     }
   }
   bool again = false;
-  if (__any_sync(FULL, special != 0.f || special_key != 0.f || zabs == INFINITY)) {  // NaNs, infinities above and NaN keys: in 64 bits
-    zabs = 0.f;
+  if (__any_sync(FULL, special != 0.f || special_key != 0.f)) {  // NaNs, infinities above and NaN keys: in 64 bits
     for (int j = 0; j < n; ++j) {
       const float v = load_logit(a, row + id0 + j), z = flip ? -v : v, b = a.bias ? a.bias[id0 + j] : 0.f;
       again = again || !(z < INFINITY) || b != b;
-      zabs = fmaxf(zabs, z == -INFINITY ? 0.f : fabsf(z));
     }
     again = seg_any(again);
   }
-  if (SCORE == DST_SCORE_SOFTMAX) {
-    zmax = value_of(seg_max(order_of(zmax)));
-    again = again || zmax == -INFINITY;  // nothing to divide by
-  }
-  // the error of a near score in units of 2^-24 of the largest one: 20 of its own steps, 2 |z| of the exponential's argument (4 |z|
-  // for softmax's difference, whose sum adds one per expert of a lane and a few), 6 |z| where a temperature rounds z; a key's own
-  // rounding comes on top where it is used
+  if (SCORE != DST_SCORE_SIGMOID) zmax = value_of(seg_max(order_of(zmax)));
+  again = again || (SCORE == DST_SCORE_SOFTMAX && zmax == -INFINITY);  // nothing to divide by
+  // The error of a near score in units of 2^-24 of the largest one. An exponential of -|z| is off by 4 and 2 |z| of itself, 2 |z| more
+  // where a temperature rounds z, and |z| exp(-|z| / 2) < 0.74: with the other steps 9 for the sigmoid and 10 for the square roots, taken
+  // as 20 (whatever z is, so masked experts of the type's lowest value do no harm). Softmax: 20, one per expert of a lane and a few
+  // for the sum, 4 |z| (10 with a temperature) for the difference, of those that count: exp(-128) is none. A key's own rounding comes on
+  // top where it is used.
   float delta = 0.f;
   if (a.bias || a.two) {
-    const float far = __uint_as_float(seg_max(__float_as_uint(zabs))) * inv_temp;  // of the finite ones
-    const float largest = SCORE == DST_SCORE_SOFTMAX ? inv_sum : SCORE == DST_SCORE_SIGMOID ? 1.f : sqrtf(far + 0.7f);
-    const float per_z = (SCORE == DST_SCORE_SOFTMAX ? 4.f : 2.f) + (inv_temp == 1.f ? 0.f : 6.f);
-    delta = largest * (20.f + (SCORE == DST_SCORE_SOFTMAX ? a.chunk + 8.f : 0.f) + per_z * far) * 0x1p-24f;
+    if (SCORE == DST_SCORE_SOFTMAX) {
+      const float far = fminf(__uint_as_float(seg_max(__float_as_uint(zabs))) * inv_temp, fabsf(zmax) * inv_temp + 128.f);
+      delta = inv_sum * (28.f + a.chunk + (inv_temp == 1.f ? 4.f : 10.f) * far) * 0x1p-24f;
+    } else {
+      delta = (SCORE == DST_SCORE_SIGMOID ? 1.f : sqrtf(fmaxf(zmax * inv_temp, 0.f) + 0.7f)) * (20.f * 0x1p-24f);
+    }
+    again = again || !(delta < INFINITY);
   }
 
   const auto key64 = [&](float z, float b) {  // softmax: without the division by the sum of all, for comparisons without a bias

@@ -40,15 +40,17 @@ def route64(logits, k, scale, renorm, score, bias, temp, groups, kept, group_sco
     s = {"softmax": lambda: torch.softmax(v, -1), "sigmoid": lambda: torch.sigmoid(v),
          "sqrtsoftplus": lambda: torch.logaddexp(v, torch.zeros_like(v)).sqrt()}[score]()
     key = s if bias is None else s + bias.double()
+    # without a bias experts rank as their logits do: the scores rise with them, though 64 bits round some alike (the sigmoid is 1 from 37 on)
+    rank = v.where(~s.isnan(), torch.nan) if bias is None else key
     size = E // groups
 
     def first(values):  # positions in descending order
         return values.sort(dim=-1, descending=True, stable=True).indices
 
-    best = key.view(T, groups, size).sort(dim=-1, descending=True).values[..., :2 if group_score == "top2" else 1].sum(-1)
+    best = (key if group_score == "top2" else rank).view(T, groups, size).sort(dim=-1, descending=True).values[..., :2 if group_score == "top2" else 1].sum(-1)
     allowed = first(best)[:, :kept].sort(dim=-1).values
     cand = (allowed[..., None] * size + torch.arange(size, device=DEV)).flatten(1)
-    ids = cand.gather(1, first(key.gather(1, cand))[:, :k])
+    ids = cand.gather(1, first(rank.gather(1, cand))[:, :k])
     w = s.gather(1, ids)
     if renorm and k > 1:
         w = w / (w.sum(-1, keepdim=True) + 1e-20)
@@ -194,6 +196,22 @@ def test_route_groups_infinities_and_nan(score):
         check_route(logits[t:t + 1], 8, score=score, groups=8, kept=2)
     if score == "sigmoid":
         _, want = route64(logits, 8, 1.0, True, score, None, 1.0, 8, 2, "top2")
+        assert np.array_equal(ids.cpu().numpy(), want)
+
+
+@gpu
+@pytest.mark.parametrize("T", [7, 5000])
+@pytest.mark.parametrize("temp", [1.0, 0.01, -0.01, 100.0])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax", "sqrtsoftplus"])
+def test_route_groups_lowest_values_and_temperatures(score, temp, T):
+    """Experts masked by the type's lowest value, which a small temperature takes past float32's range (and a negative one to the top)."""
+    g = gen(T)
+    logits = torch.randn(T, 64, generator=g, device=DEV)
+    logits[torch.rand(T, 64, generator=g, device=DEV) < 0.3] = torch.finfo(F32).min
+    bias = torch.randn(64, generator=g, device=DEV) * 0.1
+    for b, how in ((bias, "top2"), (None, "top2"), (bias, "max")):
+        w, ids = B200Ops().route(logits, 4, 1.0, score_func=score, bias=b, gate_temp=temp, n_groups=8, topk_groups=3, group_score=how)
+        _, want = route64(logits, 4, 1.0, True, score, b, temp, 8, 3, how)
         assert np.array_equal(ids.cpu().numpy(), want)
 
 
